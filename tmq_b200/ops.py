@@ -473,7 +473,8 @@ class _StatusWatch:
         self.launches = 0
 
     def note_launch(self):
-        if self.pending and self.event.query():
+        # an event may not be queried while the stream is being captured: the capture would be lost
+        if self.pending and not torch.cuda.is_current_stream_capturing() and self.event.query():
             self.pending = False
             code = int(self.host[0])
             if code != 0:
