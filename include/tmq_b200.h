@@ -245,6 +245,55 @@ int tmq_ternary_gemv_batched_bf16(const void *X, int64_t x_stride, const uint32_
 int tmq_ternary_gemv_batched_i8(const int8_t *X, int64_t x_stride, const uint32_t *const *Wt, int32_t *const *Y, int nmat,
                                 int64_t M, int64_t N, int64_t K, int64_t ldy, int *status, void *stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * 8-bit activations with scales per token and channel, plain and grouped by expert.
+ *
+ * tmq_quantize_rows: X [M][ldx] (TMQ_TYPE_*) -> codes Q int8 [M][ldq] and one scale per row:
+ *   amax = max_k |x_k|,  scale = amax / 127 (one fp32 rounding),  q_k = round-half-even(127 x_k / amax), decided exactly.
+ * Columns K .. cols - 1 of Q are set to zero (K <= cols <= ldq), the rest of a row is left alone.  amax = 0: scale 0, codes 0.  A NaN or an infinity in a row: scale NaN, codes 0
+ * (the products of that row are NaN, other rows are unaffected).  Rows of a weight matrix quantise the same way (one scale
+ * per output channel).  Any M, K, alignment; 16-byte aligned rows of X and Q with ldq % 16 == 0 and cols % 16 == 0 take the
+ * vector accesses.
+ * extends: Linear.compact_forward, tmq/tmq.py:662-688 (fp32 activations only).
+ * ------------------------------------------------------------------------------------------------ */
+#define TMQ_TYPE_F32 0
+#define TMQ_TYPE_BF16 1
+#define TMQ_TYPE_F16 2
+int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *scale, int64_t M, int64_t K, int64_t ldx, int64_t ldq,
+                      int64_t cols, void *stream);
+
+/* Y[m][n] = acc * row_scale[m] * scale[n] + bias[n],  acc = sum_k X[m][k] W[n][k] exact in int32 (K <= 131071), then fp32:
+ * (acc * row_scale) rounded, times scale plus bias in one fused multiply-add, rounded once more to y_type (TMQ_TYPE_*).
+ * row_scale [M], scale [N], bias [N]: fp32, NULL for 1 / 1 / 0.  X int8 [M][ldx], 16-byte aligned, ldx % 16 == 0, any
+ * K <= ldx (columns beyond K are not read).  Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw],
+ * 16-byte aligned, ldw % 16 == 0.  Y [M][ldy], element-aligned (16-byte aligned with ldy % 8 == 0 takes vector stores).
+ * *status: see "Status word" above.
+ * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549, and the post_scale / bias of Linear.compact_forward, tmq/tmq.py:662-688. */
+int tmq_ternary_gemm_a8(const int8_t *X, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
+                        const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
+                        void *stream);
+int tmq_gemm_i8(const int8_t *X, int64_t ldx, const float *row_scale, const int8_t *W, int64_t ldw, const float *scale,
+                const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
+                void *stream);
+
+/* Products grouped by expert: rows offsets[e] .. offsets[e + 1] - 1 of X use matrix e of the stacked weights
+ * ([groups][N] rows, the layouts above; bf16: tmq_prepack fmt 0, X bf16 with ldx % 8 == 0), scale and bias [groups][N].
+ * offsets: DEVICE array of groups + 1 boundaries, int32 or int64 (offsets_bytes = 4 or 8), read by the kernel only; groups
+ * may be empty.  Boundaries outside 0 .. M are clamped and a boundary below its predecessor is raised to it, so bad values
+ * give empty groups.  Rows outside every group are left as they were, or set to zero when zero_rest != 0.
+ * 1 <= groups <= TMQ_GROUPS_MAX.
+ * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549 (one matrix per call). */
+#define TMQ_GROUPS_MAX 512
+int tmq_ternary_gemm_grouped_bf16(const void *X, int64_t ldx, const uint32_t *Wt, const float *scale, const float *bias,
+                                  const void *offsets, int offsets_bytes, int groups, void *Y, int y_type, int64_t M,
+                                  int64_t N, int64_t K, int64_t ldy, int zero_rest, int *status, void *stream);
+int tmq_ternary_gemm_grouped_a8(const int8_t *X, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
+                                const float *bias, const void *offsets, int offsets_bytes, int groups, void *Y, int y_type,
+                                int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest, int *status, void *stream);
+int tmq_gemm_grouped_i8(const int8_t *X, int64_t ldx, const float *row_scale, const int8_t *W, int64_t ldw, const float *scale,
+                        const float *bias, const void *offsets, int offsets_bytes, int groups, void *Y, int y_type, int64_t M,
+                        int64_t N, int64_t K, int64_t ldy, int zero_rest, int *status, void *stream);
+
 /* Training forward of a quantisation-aware Linear layer with the soft staircase fused into the weight-operand load:
  *   Y[m][n] = sum_k X[m][k] * S(W[n][k]; hardness) + bias[n]
  * X bf16 [M][K] (K % 8 == 0, 16-byte aligned), W the latent fp32 weights [N][K] (16-byte aligned), bias fp32 [N] or

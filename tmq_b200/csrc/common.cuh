@@ -77,6 +77,24 @@ inline int blocks_per_sm(K kernel, int threads, size_t smem = 0) {
     return b;
 }
 
+// Launch with programmatic stream serialisation: the kernel may start while its predecessor in the stream drains and
+// must execute griddepcontrol.wait, in every block, before it touches anything the predecessor wrote or reads.
+template <typename Args>
+inline int launch_chained(void (*kernel)(const Args), const Args &a, unsigned grid, unsigned threads, size_t smem,
+                          cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kernel, a));
+}
+
 // Deterministic two-stage reduction scratch: [0] arrival counter, [256..] one fp64 partial per block.
 constexpr int kMaxPartials = 65536;
 constexpr size_t kScratchHeader = 256;

@@ -739,6 +739,257 @@ def ternary_gemv_batched(x, wts, columns, scales=None, biases=None, out_dtype=to
     return outs
 
 
+# ------------------------------------------------------------------------------------------------ 8-bit products
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # TMQ_TYPE_*
+I8_K_MAX = 131071        # int32 sums of 8-bit products are exact up to this length
+GROUPS_MAX = 512         # experts one grouped launch takes (TMQ_GROUPS_MAX)
+
+
+def _enqueue(fn, device, what, *args):
+    """fn(*args, stream) on the current stream of `device`, which is made the current device for the call."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        check(fn(*args, torch.cuda.current_stream(index).cuda_stream), what)
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, torch.cuda.current_stream(index).cuda_stream), what)
+
+
+def _vector(name, what, t, shape, device):
+    """Device pointer holder of an optional fp32 vector: (tensor or None, address or None)."""
+    if t is None:
+        return None, None
+    if tuple(t.shape) != shape:
+        raise RuntimeError(f"{name}: {what} must have shape {list(shape)}")
+    if t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+        t = t.detach().to(device=device, dtype=torch.float32).contiguous()
+    return t, t.data_ptr()
+
+
+def _rows_in(name, x, dtypes):
+    if not isinstance(x, torch.Tensor) or x.device.type != "cuda" or x.dim() != 2 or x.dtype not in dtypes:
+        raise RuntimeError(f"{name}: expected a 2-D CUDA activation tensor of type "
+                           + " / ".join(str(d).replace("torch.", "") for d in dtypes))
+    if x.shape[1] == 0:
+        raise RuntimeError(f"{name}: rows without elements")
+
+
+def _aligned_rows(x):
+    """(tensor, row stride) of rows the TMA path can read: unit column stride, 16-byte aligned rows that do not overlap.
+    Anything else is copied into such rows first."""
+    M, K = x.shape
+    esz = x.element_size()
+    lanes = 16 // esz
+    if x.stride(1) == 1 or K == 1:
+        if x.data_ptr() % 16 == 0:
+            if M == 1:
+                return x, (K + lanes - 1) // lanes * lanes
+            if x.stride(0) >= K and x.stride(0) % lanes == 0:
+                return x, x.stride(0)
+    kp = (K + lanes - 1) // lanes * lanes
+    rows = torch.empty((M, kp), dtype=x.dtype, device=x.device)
+    rows[:, :K].copy_(x)
+    return rows, kp
+
+
+def _rows_out(name, out, M, N, dtype, device):
+    """(tensor, row stride) of the result: fresh, or the caller's `out` with rows of any stride."""
+    if dtype not in _TYPES:
+        raise ValueError(f"{name}: output dtype must be float32, bfloat16 or float16")
+    if out is None:
+        return torch.empty((M, N), dtype=dtype, device=device), N
+    if out.dtype != dtype or out.device != device or out.dim() != 2 or tuple(out.shape) != (M, N) or \
+            (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+        raise RuntimeError(f"{name}: `out` must be an [M, N] tensor of the output dtype with unit column stride")
+    return out, out.stride(0) if M > 1 else N
+
+
+def quantize_rows(x, out=None):
+    """Rows of a CUDA fp32 / bf16 / fp16 matrix [M, K] -> (codes int8 [M, K], scale fp32 [M]) with
+    scale = max|row| / 127 and codes = round-half-even(127 row / max|row|), decided exactly.  A zero row gets scale 0; a row
+    that holds a NaN or an infinity gets scale NaN (and codes 0), so products of that row are NaN.  The codes are a view of
+    rows padded to a multiple of 16 bytes, the form the 8-bit products read in place.  The rows of a weight matrix are its
+    output channels: quantize_rows(weight) makes the operands of gemm_i8.  out: optional (codes, scale) to write into, codes
+    with unit column stride; padding columns of `out` are not touched."""
+    _rows_in("quantize_rows", x, (torch.float32, torch.bfloat16, torch.float16))
+    if x.stride(1) != 1 and x.shape[1] > 1:
+        x = x.contiguous()
+    M, K = x.shape
+    if out is None:
+        kp = (K + 15) // 16 * 16
+        rows = torch.empty((M, kp), dtype=torch.int8, device=x.device)
+        scale = torch.empty(M, dtype=torch.float32, device=x.device)
+        q, width = (rows if kp == K else rows[:, :K]), kp
+    else:
+        q, scale = out
+        if q.dtype != torch.int8 or q.device != x.device or tuple(q.shape) != (M, K) or (K > 1 and q.stride(1) != 1) or \
+                (M > 1 and q.stride(0) < K) or scale.dtype != torch.float32 or scale.device != x.device or \
+                tuple(scale.shape) != (M,) or not scale.is_contiguous():
+            raise RuntimeError("quantize_rows: `out` must be (int8 [M, K] with unit column stride, float32 [M])")
+        width = K
+    if M:
+        ldx = x.stride(0) if M > 1 else (K + 15) // 16 * 16
+        ldq = q.stride(0) if M > 1 else (width + 15) // 16 * 16
+        if ldx < K:                                   # expanded rows
+            x = x.contiguous()
+            ldx = K
+        _enqueue(lib().tmq_quantize_rows, x.device, "quantize_rows", x.data_ptr(), _TYPES[x.dtype], q.data_ptr(),
+                 scale.data_ptr(), M, K, ldx, ldq, width)
+    return q, scale
+
+
+def _a8_operands(name, x, row_scale):
+    """int8 rows and their scales: as given, or quantised here from floating point."""
+    _rows_in(name, x, (torch.int8, torch.float32, torch.bfloat16, torch.float16))
+    if x.dtype != torch.int8:
+        if row_scale is not None:
+            raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
+        x, row_scale = quantize_rows(x)
+    if x.shape[1] > I8_K_MAX:
+        raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
+    return x, row_scale
+
+
+def ternary_gemm_a8(x, wt, columns, row_scale=None, scale=None, bias=None, out_dtype=torch.bfloat16, out=None):
+    """Y[m][n] = row_scale[m] * scale[n] * sum_k x[m][k] T[n][k] + bias[n] with 8-bit activations and packed ternary
+    weights; the sums are exact, the scaling is fp32, the result bf16, fp16 or fp32 [M, columns].
+    x: CUDA int8 [M, K] (any row stride; row_scale fp32 [M] or None for 1), or fp32 / bf16 / fp16 [M, K], which is quantised
+    here exactly as quantize_rows does.  wt: prepack(..., FMT_I8).  scale, bias: fp32 [columns] or None.  out: optional
+    [M, columns] tensor of the output dtype whose rows may be strided.  No gradient."""
+    x, row_scale = _a8_operands("ternary_gemm_a8", x, row_scale)
+    M, K = x.shape
+    N = int(columns)
+    _check_weights("ternary_gemm_a8", wt, N, K, FMT_I8)
+    if wt.device != x.device:
+        raise RuntimeError("ternary_gemm_a8: weights on another device than the activations")
+    dev = x.device
+    rs, p_rs = _vector("ternary_gemm_a8", "row_scale", row_scale, (M,), dev)
+    sc, p_sc = _vector("ternary_gemm_a8", "scale", scale, (N,), dev)
+    bi, p_bi = _vector("ternary_gemm_a8", "bias", bias, (N,), dev)
+    y, ldy = _rows_out("ternary_gemm_a8", out, M, N, out_dtype, dev)
+    if M == 0:
+        return y
+    x, ldx = _aligned_rows(x)
+    _enqueue(lib().tmq_ternary_gemm_a8, dev, "ternary_gemm_a8", x.data_ptr(), ldx, p_rs, wt.data_ptr(), p_sc, p_bi,
+             y.data_ptr(), _TYPES[y.dtype], M, N, K, ldy, gemm_status_word(dev).data_ptr())
+    _launched(dev)
+    return y
+
+
+def _check_i8_weights(name, w, dims, device):
+    """8-bit weights are read in place: the row stride of a stack [E, N, K] / matrix [N, K], or a refusal."""
+    if w.dtype != torch.int8 or w.device != device or w.dim() != dims or w.shape[-1] == 0 or w.shape[-2] == 0:
+        raise RuntimeError(f"{name}: expected int8 weights {'[N, K]' if dims == 2 else '[experts, N, K]'} on the "
+                           "activations' device")
+    N, K = w.shape[-2:]
+    ldw = w.stride(-2) if N > 1 else (K + 15) // 16 * 16
+    ok = (K == 1 or w.stride(-1) == 1) and ldw >= K and ldw % 16 == 0 and w.data_ptr() % 16 == 0
+    if dims == 3 and w.shape[0] > 1:
+        ok = ok and w.stride(0) == N * ldw
+    if not ok:
+        raise RuntimeError(f"{name}: the weights' rows must lie one behind the other, each starting at a multiple of 16 bytes "
+                           "(pad the rows as quantize_rows does)")
+    return ldw
+
+
+def gemm_i8(x, weight, row_scale=None, scale=None, bias=None, out_dtype=torch.bfloat16, out=None):
+    """ternary_gemm_a8 for 8-bit weights: weight int8 [N, K] with rows that start at multiples of 16 bytes (what
+    quantize_rows returns), scale fp32 [N] per channel.  Everything else as there."""
+    x, row_scale = _a8_operands("gemm_i8", x, row_scale)
+    M, K = x.shape
+    dev = x.device
+    ldw = _check_i8_weights("gemm_i8", weight, 2, dev)
+    N = weight.shape[0]
+    if weight.shape[1] != K:
+        raise RuntimeError("gemm_i8: activation width does not match the weights")
+    rs, p_rs = _vector("gemm_i8", "row_scale", row_scale, (M,), dev)
+    sc, p_sc = _vector("gemm_i8", "scale", scale, (N,), dev)
+    bi, p_bi = _vector("gemm_i8", "bias", bias, (N,), dev)
+    y, ldy = _rows_out("gemm_i8", out, M, N, out_dtype, dev)
+    if M == 0:
+        return y
+    x, ldx = _aligned_rows(x)
+    _enqueue(lib().tmq_gemm_i8, dev, "gemm_i8", x.data_ptr(), ldx, p_rs, weight.data_ptr(), ldw, p_sc, p_bi, y.data_ptr(),
+             _TYPES[y.dtype], M, N, K, ldy, gemm_status_word(dev).data_ptr())
+    _launched(dev)
+    return y
+
+
+def _check_offsets(name, offsets, groups, device):
+    if offsets.dtype not in (torch.int32, torch.int64) or offsets.device != device or offsets.dim() != 1 or \
+            offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
+        raise RuntimeError(f"{name}: offsets must be a contiguous int32 or int64 tensor of experts + 1 boundaries on the "
+                           "activations' device")
+    if not 1 <= groups <= GROUPS_MAX:
+        raise RuntimeError(f"{name}: 1 .. {GROUPS_MAX} experts")
+
+
+def ternary_gemm_grouped(x, wts, columns, offsets, row_scale=None, scales=None, biases=None, out_dtype=torch.bfloat16,
+                         out=None):
+    """Products grouped by expert: rows offsets[e] .. offsets[e + 1] - 1 of x are multiplied with expert e's packed ternary
+    matrix.  x: CUDA [M, K], rows sorted by expert; bf16 with wts of FMT_BF16 (fp32 accumulation), or int8 with wts of
+    FMT_I8 and row_scale fp32 [M] (quantize_rows makes both).  wts: int32 [experts, columns, row words], the stack of the
+    experts' prepack() results.  offsets: experts + 1 boundaries, int32 or int64, on the device; they are not read by the
+    host, so the call neither synchronises nor depends on the counts, and a captured call follows the boundaries of each
+    replay.  Groups may be empty.  scales, biases: fp32 [experts, columns] or None.  Rows outside every group are zero in a
+    fresh result and left as they were in `out`.  Boundaries outside 0 .. M or out of order give empty or shortened groups.
+    No gradient."""
+    _rows_in("ternary_gemm_grouped", x, (torch.bfloat16, torch.int8))
+    i8 = x.dtype == torch.int8
+    M, K = x.shape
+    N = int(columns)
+    dev = x.device
+    if not isinstance(wts, torch.Tensor) or wts.dim() != 3 or wts.device != dev or not wts.is_contiguous():
+        raise RuntimeError("ternary_gemm_grouped: expected the stacked prepacked weights [experts, columns, row words] on the "
+                           "activations' device")
+    E = wts.shape[0]
+    _check_offsets("ternary_gemm_grouped", offsets, E, dev)
+    _check_weights("ternary_gemm_grouped", wts[0], N, K, FMT_I8 if i8 else FMT_BF16)
+    if i8 and K > I8_K_MAX:
+        raise RuntimeError(f"ternary_gemm_grouped: at most {I8_K_MAX} columns (int32 sums)")
+    if not i8 and row_scale is not None:
+        raise RuntimeError("ternary_gemm_grouped: row_scale belongs to int8 activations")
+    rs, p_rs = _vector("ternary_gemm_grouped", "row_scale", row_scale, (M,), dev)
+    sc, p_sc = _vector("ternary_gemm_grouped", "scales", scales, (E, N), dev)
+    bi, p_bi = _vector("ternary_gemm_grouped", "biases", biases, (E, N), dev)
+    y, ldy = _rows_out("ternary_gemm_grouped", out, M, N, out_dtype, dev)
+    if M == 0:
+        return y
+    x, ldx = _aligned_rows(x)
+    head = (x.data_ptr(), ldx) + ((p_rs,) if i8 else ()) + (wts.data_ptr(), p_sc, p_bi)
+    _enqueue(lib().tmq_ternary_gemm_grouped_a8 if i8 else lib().tmq_ternary_gemm_grouped_bf16, dev, "ternary_gemm_grouped",
+             *head, offsets.data_ptr(), offsets.element_size(), E, y.data_ptr(), _TYPES[y.dtype], M, N, K, ldy,
+             1 if out is None else 0, gemm_status_word(dev).data_ptr())
+    _launched(dev)
+    return y
+
+
+def gemm_i8_grouped(x, weights, offsets, row_scale=None, scales=None, biases=None, out_dtype=torch.bfloat16, out=None):
+    """ternary_gemm_grouped for 8-bit weights: weights int8 [experts, N, K] whose rows lie one behind the other and start at
+    multiples of 16 bytes; x int8 [M, K] with row_scale fp32 [M].  Everything else as there."""
+    _rows_in("gemm_i8_grouped", x, (torch.int8,))
+    M, K = x.shape
+    dev = x.device
+    ldw = _check_i8_weights("gemm_i8_grouped", weights, 3, dev)
+    E, N = weights.shape[:2]
+    _check_offsets("gemm_i8_grouped", offsets, E, dev)
+    if weights.shape[2] != K or K > I8_K_MAX:
+        raise RuntimeError("gemm_i8_grouped: activation width does not match the weights or exceeds the int32 sums")
+    rs, p_rs = _vector("gemm_i8_grouped", "row_scale", row_scale, (M,), dev)
+    sc, p_sc = _vector("gemm_i8_grouped", "scales", scales, (E, N), dev)
+    bi, p_bi = _vector("gemm_i8_grouped", "biases", biases, (E, N), dev)
+    y, ldy = _rows_out("gemm_i8_grouped", out, M, N, out_dtype, dev)
+    if M == 0:
+        return y
+    x, ldx = _aligned_rows(x)
+    _enqueue(lib().tmq_gemm_grouped_i8, dev, "gemm_i8_grouped", x.data_ptr(), ldx, p_rs, weights.data_ptr(), ldw, p_sc, p_bi,
+             offsets.data_ptr(), offsets.element_size(), E, y.data_ptr(), _TYPES[y.dtype], M, N, K, ldy,
+             1 if out is None else 0, gemm_status_word(dev).data_ptr())
+    _launched(dev)
+    return y
+
+
 def qat_linear_forward(x, weight, bias, hardness):
     """Training forward of a quantisation-aware Linear layer, x @ S(weight)^T + bias, with the soft staircase S evaluated
     inside the tensor-core GEMM's operand producers (never materialised).  x: CUDA bf16 [..., K] with K % 8 == 0;
