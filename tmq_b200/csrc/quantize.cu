@@ -19,14 +19,14 @@ struct QuantArgs {
     int8_t *Q;
     float *scale;
     long long M, K, ldx, ldq, cols;        // cols >= K: columns written
+    int vstore;
 };
 
-// One row per TPR threads, 256 threads per block.  VEC: elements of one 16-byte load (1: the row is not 16-byte aligned
-// and is read element by element).  CH: chunks of VEC elements a thread holds.
-template <typename T, int TPR, int VEC, int CH>
+// One row per TPR threads, 256 threads per block, CH vectors held per thread; the rest of a longer row is read twice.
+template <typename T, bool VLOAD, int TPR, int CH>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
-    constexpr int ROWS = 256 / TPR;
-    __shared__ float red[8];
+    constexpr int ROWS = 256 / TPR, V = QuantType<T>::V;
+    __shared__ uint32_t red[8];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int t = threadIdx.x % TPR;
@@ -35,56 +35,74 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
     const T *x = reinterpret_cast<const T *>(a.X) + (live ? m : 0) * a.ldx;
     const long long K = live ? a.K : 0;
 
-    QuantChunk<T, VEC> held[CH];
-    float amax = 0.0f;
-    bool bad = false;
+    QuantVec<T> held[CH];
+    uint32_t peak = 0;
 #pragma unroll
-    for (int c = 0; c < CH; c++) held[c].load(x, ((long long)c * TPR + t) * VEC, K);
+    for (int c = 0; c < CH; c++) held[c].template load<VLOAD>(x, (c * TPR + t) * V, K);
 #pragma unroll
-    for (int c = 0; c < CH; c++) held[c].peak(amax, bad);
-    for (long long k = ((long long)CH * TPR + t) * VEC; k < K; k += (long long)TPR * VEC) {
-        QuantChunk<T, VEC> v;
-        v.load(x, k, K);
-        v.peak(amax, bad);
+    for (int c = 0; c < CH; c++) held[c].peak(peak);
+    for (long long k = (CH * TPR + t) * V; k < K; k += TPR * V) {
+        QuantVec<T> v;
+        v.template load<VLOAD>(x, k, K);
+        v.peak(peak);
     }
-    if (bad) amax = __int_as_float(0x7f800000);          // one non-finite value marks the row
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    peak = __reduce_max_sync(0xffffffffu, QuantType<T>::fold(peak));
     if (TPR > 32) {
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = amax;
+        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = peak;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 8; w++) amax = fmaxf(amax, red[w]);
+        for (int w = 0; w < 8; w++) peak = max(peak, red[w]);
     }
     if (!live) return;
-    const RowQuant rq(amax);
+    const RowQuant<T> rq(peak);
     if (t == 0) a.scale[m] = rq.scale;
     int8_t *q = a.Q + m * a.ldq;
+    auto put = [&](const QuantVec<T> &v, long long k) {
+        if (k >= a.cols) return;
+        uint32_t c[V / 4];
+        v.codes(rq, c);
+        if (a.vstore) {                                  // cols is a multiple of V: the whole vector exists
+            if (V == 8) *reinterpret_cast<uint2 *>(q + k) = make_uint2(c[0], c[V / 4 - 1]);
+            else *reinterpret_cast<uint32_t *>(q + k) = c[0];
+        } else {
 #pragma unroll
-    for (int c = 0; c < CH; c++) held[c].store(q, ((long long)c * TPR + t) * VEC, a.K, a.cols, rq);
-    for (long long k = ((long long)CH * TPR + t) * VEC; k < a.cols; k += (long long)TPR * VEC) {
-        QuantChunk<T, VEC> v;
-        v.load(x, k, a.K);
-        v.store(q, k, a.K, a.cols, rq);
+            for (int i = 0; i < V; i++)
+                if (k + i < a.cols) q[k + i] = (int8_t)(c[i / 4] >> (8 * (i & 3)));
+        }
+    };
+#pragma unroll
+    for (int c = 0; c < CH; c++) put(held[c], (c * TPR + t) * V);
+    for (long long k = (CH * TPR + t) * V; k < a.cols; k += TPR * V) {
+        QuantVec<T> v;
+        v.template load<VLOAD>(x, k, a.K);
+        put(v, k);
     }
 }
 
-template <typename T, int TPR, int VEC, int CH>
+template <typename T, bool VLOAD, int TPR, int CH>
 static int launch_quantize(const QuantArgs &a, cudaStream_t st) {
     const long long rows = 256 / TPR, grid = (a.M + rows - 1) / rows;
     if (grid > 0x7FFFFFFF) return TMQ_ERR_UNSUPPORTED;
-    return launch_chained(quantize_rows_kernel<T, TPR, VEC, CH>, a, (unsigned)grid, 256, 0, st);
+    return launch_chained(quantize_rows_kernel<T, VLOAD, TPR, CH>, a, (unsigned)grid, 256, 0, st);
+}
+
+template <typename T, bool VLOAD>
+static int dispatch_width(const QuantArgs &a, cudaStream_t st) {
+    constexpr int V = QuantType<T>::V;
+    // short rows: one warp each when there are enough of them to fill the machine
+    if (a.K <= 32 * V * 4 && a.M >= 8 * kNumSMs) return launch_quantize<T, VLOAD, 32, 4>(a, st);
+    if (a.K <= 256 * V) return launch_quantize<T, VLOAD, 256, 1>(a, st);
+    if (a.K <= 256 * V * 2) return launch_quantize<T, VLOAD, 256, 2>(a, st);
+    if (a.K <= 256 * V * 4) return launch_quantize<T, VLOAD, 256, 4>(a, st);
+    return launch_quantize<T, VLOAD, 256, 8>(a, st);
 }
 
 template <typename T>
-static int dispatch_quantize(const QuantArgs &a, cudaStream_t st) {
-    constexpr int V = 16 / sizeof(T);
-    const bool vec = aligned(a.X, 16) && (a.ldx * (long long)sizeof(T)) % 16 == 0 && aligned(a.Q, 16) && a.ldq % 16 == 0 &&
-                     a.cols % 16 == 0;
-    if (!vec) return launch_quantize<T, 256, 1, 8>(a, st);
-    if (a.K <= 32 * V * 4 && a.M >= 8 * kNumSMs) return launch_quantize<T, 32, V, 4>(a, st);
-    if (a.K <= 256 * V * 2) return launch_quantize<T, 256, V, 2>(a, st);
-    return launch_quantize<T, 256, V, 8>(a, st);
+static int dispatch_quantize(QuantArgs a, cudaStream_t st) {
+    constexpr int V = QuantType<T>::V;
+    a.vstore = aligned(a.Q, V) && a.ldq % V == 0 && a.cols % V == 0;
+    if (aligned(a.X, 16) && (a.ldx * (long long)sizeof(T)) % 16 == 0) return dispatch_width<T, true>(a, st);
+    return dispatch_width<T, false>(a, st);
 }
 
 }  // namespace tmq
@@ -97,7 +115,7 @@ extern "C" int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *sc
     if (M == 0) return TMQ_OK;
     if (!X || !Q || !scale) return TMQ_ERR_ARG;
     if (!aligned(X, x_type == TMQ_TYPE_F32 ? 4 : 2) || !aligned(scale, 4)) return TMQ_ERR_ALIGN;
-    const QuantArgs a = {X, Q, scale, M, K, ldx, ldq, cols};
+    const QuantArgs a = {X, Q, scale, M, K, ldx, ldq, cols, 0};
     if (x_type == TMQ_TYPE_F32) return dispatch_quantize<float>(a, (cudaStream_t)stream);
     if (x_type == TMQ_TYPE_BF16) return dispatch_quantize<__nv_bfloat16>(a, (cudaStream_t)stream);
     return dispatch_quantize<__half>(a, (cudaStream_t)stream);

@@ -30,7 +30,7 @@ enum { W_TERNARY_BF16 = 0, W_TERNARY_I8 = 1, W_DENSE_I8 = 2 };
 
 constexpr int kTileC = 128;          // channels of a unit (MMA M)
 constexpr int kOpRow = 128;          // bytes of one operand row per k-block: 64 bf16 or 128 int8
-constexpr int kBoxRows = 32;         // rows of one activation box
+constexpr int kRowStep = 32;         // granularity of a unit's MMA N
 constexpr int kMaxGroups = TMQ_GROUPS_MAX;
 constexpr int kDecodeWarps = 8;
 
@@ -54,6 +54,8 @@ struct ScaledCfg {
     static constexpr int A_BYTES = TA ? 0 : kTileC * kOpRow;
     static constexpr int B_BYTES = BN * kOpRow;
     static constexpr int RAW_BYTES = kTileC * RAW_ROW;
+    // activations arrive as one box of BN rows, or, for a unit of at most half of that, as one or two small boxes
+    static constexpr int SMALL = BN > 128 ? 64 : 32;
     static constexpr int ACC_BUFS = (TA && BN > 128) ? 1 : 2;
     static constexpr int A_COLS = kOpRow / 4;
     static constexpr int A_BASE = ACC_BUFS * BN;
@@ -161,7 +163,8 @@ __device__ __forceinline__ void store_eight(void *Y, int y_type, long long i, co
 
 template <int WK, int BN>
 __global__ void __launch_bounds__(ScaledCfg<WK, BN>::THREADS, 1)
-scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const ScaledArgs a) {
+scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_small,
+                   const __grid_constant__ CUtensorMap tmap_w, const ScaledArgs a) {
     using C = ScaledCfg<WK, BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -191,6 +194,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         }
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tmap_x);
+        ptx::prefetch_tensormap(&tmap_small);
         ptx::prefetch_tensormap(&tmap_w);
     }
     if (warp == 1) {
@@ -213,9 +217,10 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
                 const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
-                const int boxes = (q.rows + kBoxRows - 1) / kBoxRows;
+                const bool whole = q.rows > BN / 2;
+                const int rows = whole ? BN : q.rows > C::SMALL ? 2 * C::SMALL : C::SMALL;
                 const int wrow = (int)(q.e * a.N) + q.n0;
-                const uint32_t bytes = (uint32_t)(boxes * kBoxRows * kOpRow + (C::DENSE ? C::A_BYTES : C::RAW_BYTES));
+                const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : C::RAW_BYTES));
                 for (int kb = 0; kb < nkb; kb++, it++) {
                     const int s = it % C::STAGES;
                     const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
@@ -224,9 +229,10 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                     ptx::mbar_arrive_expect_tx(full + s, bytes);
                     if (C::DENSE) ptx::tma_load_2d(smem + C::A_OFF + s * C::A_BYTES, &tmap_w, full + s, kb * C::BK, wrow);
                     else ptx::tma_load_2d(smem + C::RAW_OFF + s * C::RAW_BYTES, &tmap_w, full + s, kb * (C::RAW_ROW / 4), wrow);
-                    for (int b = 0; b < boxes; b++)
-                        ptx::tma_load_2d(smem + C::B_OFF + s * C::B_BYTES + b * (kBoxRows * kOpRow), &tmap_x, full + s, kb * C::BK,
-                                         q.row0 + b * kBoxRows);
+                    uint8_t *dst = smem + C::B_OFF + s * C::B_BYTES;
+                    ptx::tma_load_2d(dst, whole ? &tmap_x : &tmap_small, full + s, kb * C::BK, q.row0);
+                    if (!whole && rows > C::SMALL)
+                        ptx::tma_load_2d(dst + C::SMALL * kOpRow, &tmap_small, full + s, kb * C::BK, q.row0 + C::SMALL);
                 }
             }
         }
@@ -237,7 +243,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x, ti++) {
                 const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
-                const uint32_t n_mma = (uint32_t)((q.rows + kBoxRows - 1) / kBoxRows * kBoxRows);
+                const uint32_t n_mma = (uint32_t)((q.rows + kRowStep - 1) / kRowStep * kRowStep);
                 const uint32_t idesc = ((C::I8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((n_mma >> 3) << 17) | ((128u >> 4) << 24);
                 const int buf = C::ACC_BUFS == 2 ? (ti & 1) : 0;
                 const uint32_t use = (uint32_t)(C::ACC_BUFS == 2 ? (ti >> 1) : ti);
@@ -415,9 +421,11 @@ template <int WK, int BN>
 static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     using C = ScaledCfg<WK, BN>;
     const ScaledArgs &a = p.a;
-    CUtensorMap mx, mw;
-    const bool okx = make_map_2d(&mx, C::I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.X, (uint64_t)a.K,
-                                 (uint64_t)a.M, (uint64_t)p.ldx * (C::I8 ? 1 : 2), C::BK, kBoxRows, CU_TENSOR_MAP_SWIZZLE_128B);
+    CUtensorMap mx, ms, mw;
+    const CUtensorMapDataType xt = C::I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const uint64_t xpitch = (uint64_t)p.ldx * (C::I8 ? 1 : 2);
+    const bool okx = make_map_2d(&mx, xt, p.X, (uint64_t)a.K, (uint64_t)a.M, xpitch, C::BK, BN, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                     make_map_2d(&ms, xt, p.X, (uint64_t)a.K, (uint64_t)a.M, xpitch, C::BK, C::SMALL, CU_TENSOR_MAP_SWIZZLE_128B);
     const uint64_t wrows = (uint64_t)a.groups * (uint64_t)a.N;
     const bool okw = C::DENSE
         ? make_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.W, (uint64_t)a.K, wrows, (uint64_t)p.ldw, C::BK, kTileC,
@@ -441,7 +449,7 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, scaled_gemm_kernel<WK, BN>, mx, mw, a));
+    return cuda_status(cudaLaunchKernelEx(&cfg, scaled_gemm_kernel<WK, BN>, mx, ms, mw, a));
 }
 
 template <int WK>

@@ -750,10 +750,12 @@ def _enqueue(fn, device, what, *args):
     """fn(*args, stream) on the current stream of `device`, which is made the current device for the call."""
     index = device.index
     if torch.cuda.current_device() == index:
-        check(fn(*args, torch.cuda.current_stream(index).cuda_stream), what)
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            check(fn(*args, torch.cuda.current_stream(index).cuda_stream), what)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc, what)
 
 
 def _vector(name, what, t, shape, device):
