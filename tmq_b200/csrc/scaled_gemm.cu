@@ -10,7 +10,8 @@
 //   * The group boundaries stay on the device.  Every CTA scans them into a table of tile counts in shared memory
 //     (clamped to the rows that exist and made non-decreasing: bad boundaries give empty groups, never a bad address) and
 //     walks the units u = CTA, CTA + grid, ... through it.
-//   * Roles: warp 0 TMA, warp 1 MMA issue, then eight decode warps (packed weights only), four epilogue warps.  Decoded
+//   * Roles: warp 0 TMA of the activations (and 8-bit weights), warp 1 MMA issue, warp 2 TMA of the packed weights, then
+//     eight decode warps (packed weights only) and four epilogue warps.  Decoded
 //     weights go to tensor memory (the MMA reads its A operand there) except for int8 tiles of 256 rows, whose two
 //     accumulators fill tensor memory: those are decoded into shared memory.  8-bit weights need no decode, TMA writes
 //     them where the MMA reads them.
@@ -50,10 +51,16 @@ struct ScaledCfg {
     static constexpr bool TA = WK == W_TERNARY_BF16 || (WK == W_TERNARY_I8 && BN <= 128);   // A operand in tensor memory
     static constexpr int BK = I8 ? 128 : 64;
     static constexpr int RAW_ROW = DENSE ? 0 : I8 ? 32 : 16;                  // packed bytes per channel and k-block
+    // Packed words come RAWK k-blocks per box: a box costs the TMA unit about four cycles a row whatever its width (one
+    // k-block per box measured 280 ns per k-block at any row count).  Rows of 128 / 64 bytes with the swizzle of that
+    // width, so the decode warps' 16-byte reads meet no bank conflicts.
+    static constexpr int RAWK = DENSE ? 1 : (TA ? 4 : 2);
+    static constexpr int RAW_PITCH = RAWK * RAW_ROW;
+    static constexpr int RAW_STAGES = DENSE ? 0 : !TA ? 2 : BN > 128 ? 2 : 4;
     static constexpr int STAGES = DENSE ? (BN > 128 ? 4 : BN > 64 ? 6 : 8) : BN > 128 ? (TA ? 6 : 4) : 8;
     static constexpr int A_BYTES = TA ? 0 : kTileC * kOpRow;
     static constexpr int B_BYTES = BN * kOpRow;
-    static constexpr int RAW_BYTES = kTileC * RAW_ROW;
+    static constexpr int RAW_BYTES = kTileC * RAW_PITCH;
     // activations arrive as one box of BN rows, or, for a unit of at most half of that, as one or two small boxes
     static constexpr int SMALL = BN > 128 ? 64 : 32;
     static constexpr int ACC_BUFS = (TA && BN > 128) ? 1 : 2;
@@ -62,13 +69,13 @@ struct ScaledCfg {
     static constexpr int TMEM_NEED = A_BASE + (TA ? STAGES * A_COLS : 0);
     static constexpr int TMEM_COLS = TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
     static_assert(TMEM_NEED <= 512, "tensor memory exceeded");
-    static constexpr int FIRST_EPI = DENSE ? 2 : 2 + kDecodeWarps;
+    static constexpr int FIRST_EPI = DENSE ? 4 : 4 + kDecodeWarps;
     static constexpr int THREADS = (FIRST_EPI + 4) * 32;
     // shared memory
     static constexpr int A_OFF = 0;
     static constexpr int B_OFF = A_OFF + STAGES * A_BYTES;
     static constexpr int RAW_OFF = B_OFF + STAGES * B_BYTES;
-    static constexpr int STAGE_OFF = RAW_OFF + STAGES * RAW_BYTES;            // 4 x 2 KB transposition areas
+    static constexpr int STAGE_OFF = RAW_OFF + RAW_STAGES * RAW_BYTES;            // 4 x 2 KB transposition areas
     static constexpr int RS_OFF = STAGE_OFF + 4 * 2048;                      // 4 x BN row scales
     static constexpr int BAR_OFF = RS_OFF + 4 * BN * 4;
     static constexpr int TAB_OFF = BAR_OFF + 512;                             // begin[groups + 1], tiles[groups + 1]
@@ -171,7 +178,9 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);         // TMA bytes landed
     uint64_t *ready = full + C::STAGES;                                       // weights decoded
     uint64_t *empty = ready + C::STAGES;
-    uint64_t *acc_full = empty + C::STAGES;                                   // [2]
+    uint64_t *raw_full = empty + C::STAGES;                                   // packed words landed
+    uint64_t *raw_empty = raw_full + C::RAW_STAGES;
+    uint64_t *acc_full = raw_empty + C::RAW_STAGES;                           // [2]
     uint64_t *acc_empty = acc_full + 2;                                       // [2]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
     int *begin = reinterpret_cast<int *>(smem + C::TAB_OFF);
@@ -187,6 +196,10 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             ptx::mbar_init(full + s, 1);
             ptx::mbar_init(ready + s, 4);
             ptx::mbar_init(empty + s, 1);
+        }
+        for (int s = 0; s < C::RAW_STAGES; s++) {
+            ptx::mbar_init(raw_full + s, 1);
+            ptx::mbar_init(raw_empty + s, kDecodeWarps);
         }
         for (int b = 0; b < 2; b++) {
             ptx::mbar_init(acc_full + b, 1);
@@ -220,7 +233,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                 const bool whole = q.rows > BN / 2;
                 const int rows = whole ? BN : q.rows > C::SMALL ? 2 * C::SMALL : C::SMALL;
                 const int wrow = (int)(q.e * a.N) + q.n0;
-                const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : C::RAW_BYTES));
+                const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : 0));
                 for (int kb = 0; kb < nkb; kb++, it++) {
                     const int s = it % C::STAGES;
                     const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
@@ -228,7 +241,6 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                     if (!ok) break;
                     ptx::mbar_arrive_expect_tx(full + s, bytes);
                     if (C::DENSE) ptx::tma_load_2d(smem + C::A_OFF + s * C::A_BYTES, &tmap_w, full + s, kb * C::BK, wrow);
-                    else ptx::tma_load_2d(smem + C::RAW_OFF + s * C::RAW_BYTES, &tmap_w, full + s, kb * (C::RAW_ROW / 4), wrow);
                     uint8_t *dst = smem + C::B_OFF + s * C::B_BYTES;
                     ptx::tma_load_2d(dst, whole ? &tmap_x : &tmap_small, full + s, kb * C::BK, q.row0);
                     if (!whole && rows > C::SMALL)
@@ -281,60 +293,91 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                 __syncwarp();
             }
         }
-    } else if (warp < C::FIRST_EPI) {
-        // ---------------------------------------------------------------- decode: two sets of four warps, alternate k-blocks
-        const int quarter = warp & 3, set = (warp - 2) >> 2;
-        const int row = quarter * 32 + lane;
-        bool ok = healthy;
-        int it = 0;
-        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            for (int kb = 0; kb < nkb; kb++, it++) {
-                if ((it & 1) != set) continue;
-                const int s = it % C::STAGES;
-                const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
-                ok = ptx::mbar_wait_warp(full + s, ph, a.status);
-                if (!ok) break;
-                const uint8_t *raw = smem + C::RAW_OFF + s * C::RAW_BYTES + row * C::RAW_ROW;
-                uint32_t cols[32];                       // the row's 128 operand bytes, K ascending
-                if (C::I8) {
-                    const uint4 p0 = *reinterpret_cast<const uint4 *>(raw);
-                    const uint4 p1 = *reinterpret_cast<const uint4 *>(raw + 16);
-                    const uint32_t words[8] = {p0.x, p0.y, p0.z, p0.w, p1.x, p1.y, p1.z, p1.w};
-#pragma unroll
-                    for (int wi = 0; wi < 8; wi++) {
-                        uint32_t r[4];
-                        decode_word_i8(words[wi], r);
-#pragma unroll
-                        for (int j = 0; j < 4; j++) cols[4 * wi + j] = r[j];
-                    }
-                } else {
-                    const uint4 p = *reinterpret_cast<const uint4 *>(raw);
-                    const uint32_t words[4] = {p.x, p.y, p.z, p.w};
-#pragma unroll
-                    for (int wi = 0; wi < 4; wi++) {
-                        uint32_t r[8];
-                        decode_word_bf16(words[wi], r);
-#pragma unroll
-                        for (int j = 0; j < 8; j++) cols[8 * wi + j] = r[j];
-                    }
+    } else if (warp == 2) {
+        // ---------------------------------------------------------------- TMA producer of the packed words
+        if (!C::DENSE && lane == 0 && healthy) {
+            int rit = 0, e = 0;
+            bool ok = true;
+            for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
+                const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
+                const int wrow = (int)(q.e * a.N) + q.n0;
+                for (int kb = 0; kb < nkb; kb += C::RAWK, rit++) {
+                    const int s = rit % (C::RAW_STAGES + C::DENSE);
+                    const uint32_t ph = (uint32_t)(rit / (C::RAW_STAGES + C::DENSE)) & 1u;
+                    ok = ptx::mbar_wait(raw_empty + s, ph ^ 1u, a.status);
+                    if (!ok) break;
+                    ptx::mbar_arrive_expect_tx(raw_full + s, (uint32_t)C::RAW_BYTES);
+                    ptx::tma_load_2d(smem + C::RAW_OFF + s * C::RAW_BYTES, &tmap_w, raw_full + s, kb * (C::RAW_ROW / 4), wrow);
                 }
-                if (C::TA) {
-                    ptx::tmem_st_x32(tmem_base + ((uint32_t)(quarter * 32) << 16) + C::A_BASE + (uint32_t)(s * C::A_COLS), cols);
-                    ptx::tmem_st_wait();
-                    ptx::tc_fence_before_sync();
-                } else {
-                    uint8_t *arow = smem + C::A_OFF + s * C::A_BYTES + row * kOpRow;
-#pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        *reinterpret_cast<uint4 *>(arow + ((c ^ (row & 7)) << 4)) =
-                            make_uint4(cols[4 * c], cols[4 * c + 1], cols[4 * c + 2], cols[4 * c + 3]);
-                    ptx::fence_proxy_async_smem();
-                }
-                __syncwarp();
-                if (lane == 0) ptx::mbar_arrive(ready + s);
             }
         }
-    } else {
+    } else if (!C::DENSE && warp >= 4 && warp < C::FIRST_EPI) {
+        // ---------------------------------------------------------------- decode: two sets of four warps, alternate k-blocks
+        const int quarter = warp & 3, set = (warp - 4) >> 2;
+        const int row = quarter * 32 + lane;
+        bool ok = healthy;
+        int it = 0, rit = 0;
+        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
+            for (int kb0 = 0; kb0 < nkb && ok; kb0 += C::RAWK, rit++) {
+                const int rs = rit % (C::RAW_STAGES + C::DENSE);
+                ok = ptx::mbar_wait_warp(raw_full + rs, (uint32_t)(rit / (C::RAW_STAGES + C::DENSE)) & 1u, a.status);
+                if (!ok) break;
+                const uint8_t *raw = smem + C::RAW_OFF + rs * C::RAW_BYTES + row * C::RAW_PITCH;
+                const int left = nkb - kb0 < C::RAWK ? nkb - kb0 : C::RAWK;
+                for (int j = (it & 1) ^ set; j < left; j += 2) {
+                    const int s = (it + j) % C::STAGES;
+                    const uint32_t ph = (uint32_t)((it + j) / C::STAGES) & 1u;
+                    uint4 p[C::I8 ? 2 : 1];
+#pragma unroll
+                    for (int h = 0; h < (C::I8 ? 2 : 1); h++) {
+                        const int c = (C::I8 ? 2 * j : j) + h;
+                        p[h] = *reinterpret_cast<const uint4 *>(raw + ((c ^ (C::RAW_PITCH == 128 ? row & 7 : (row >> 1) & 3)) << 4));
+                    }
+                    uint32_t cols[32];                   // the row's 128 operand bytes, K ascending
+                    if (C::I8) {
+                        const uint32_t words[8] = {p[0].x, p[0].y, p[0].z, p[0].w, p[C::I8].x, p[C::I8].y, p[C::I8].z, p[C::I8].w};
+#pragma unroll
+                        for (int wi = 0; wi < 8; wi++) {
+                            uint32_t r[4];
+                            decode_word_i8(words[wi], r);
+#pragma unroll
+                            for (int x = 0; x < 4; x++) cols[4 * wi + x] = r[x];
+                        }
+                    } else {
+                        const uint32_t words[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
+#pragma unroll
+                        for (int wi = 0; wi < 4; wi++) {
+                            uint32_t r[8];
+                            decode_word_bf16(words[wi], r);
+#pragma unroll
+                            for (int x = 0; x < 8; x++) cols[8 * wi + x] = r[x];
+                        }
+                    }
+                    // the MMAs that read this operand slot last are done
+                    ok = ptx::mbar_wait_warp(empty + s, ph ^ 1u, a.status);
+                    if (!ok) break;
+                    if (C::TA) {
+                        ptx::tc_fence_after_sync();
+                        ptx::tmem_st_x32(tmem_base + ((uint32_t)(quarter * 32) << 16) + C::A_BASE + (uint32_t)(s * C::A_COLS), cols);
+                        ptx::tmem_st_wait();
+                        ptx::tc_fence_before_sync();
+                    } else {
+                        uint8_t *arow = smem + C::A_OFF + s * C::A_BYTES + row * kOpRow;
+#pragma unroll
+                        for (int c = 0; c < 8; c++)
+                            *reinterpret_cast<uint4 *>(arow + ((c ^ (row & 7)) << 4)) =
+                                make_uint4(cols[4 * c], cols[4 * c + 1], cols[4 * c + 2], cols[4 * c + 3]);
+                        ptx::fence_proxy_async_smem();
+                    }
+                    __syncwarp();
+                    if (lane == 0) ptx::mbar_arrive(ready + s);
+                }
+                it += left;
+                __syncwarp();
+                if (ok && lane == 0) ptx::mbar_arrive(raw_empty + rs);
+            }
+        }
+    } else if (warp >= C::FIRST_EPI) {
         // ---------------------------------------------------------------- epilogue
         const int quarter = warp & 3;
         float *stage = reinterpret_cast<float *>(smem + C::STAGE_OFF) + (warp - C::FIRST_EPI) * 512;
@@ -369,11 +412,22 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(acc_empty + buf);
                 }
+                float f[16];
 #pragma unroll
                 for (int j = 0; j < 16; j++) {
                     const float acc = C::I8 ? __int2float_rn((int)v[j]) : __uint_as_float(v[j]);
-                    stage[j * 32 + lane] = fmaf(__fmul_rn(acc, rs[c + j]), sc, bi);
+                    f[j] = fmaf(__fmul_rn(acc, rs[c + j]), sc, bi);
                 }
+                if (!vec_rows) {                         // rows that allow no vectors: a warp writes 32 neighbouring channels
+                    if (n < a.N) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            if (c + j < q.rows) store_one(a.Y, a.y_type, (long long)(q.row0 + c + j) * a.ldy + n, f[j]);
+                    }
+                    continue;
+                }
+#pragma unroll
+                for (int j = 0; j < 16; j++) stage[j * 32 + lane] = f[j];
                 __syncwarp();
                 const int cg = (lane & 3) * 8, nb = q.n0 + quarter * 32 + cg;
 #pragma unroll
@@ -382,11 +436,11 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                     if (c + p < q.rows && nb < a.N) {
                         const float4 lo = *reinterpret_cast<const float4 *>(stage + p * 32 + cg);
                         const float4 hi = *reinterpret_cast<const float4 *>(stage + p * 32 + cg + 4);
-                        const float f[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                        const float o[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
                         const long long i = (long long)(q.row0 + c + p) * a.ldy + nb;
-                        if (vec_rows && nb + 8 <= a.N) store_eight(a.Y, a.y_type, i, f);
+                        if (nb + 8 <= a.N) store_eight(a.Y, a.y_type, i, o);
                         else
-                            for (int x = 0; x < 8 && nb + x < a.N; x++) store_one(a.Y, a.y_type, i + x, f[x]);
+                            for (int x = 0; x < 8 && nb + x < a.N; x++) store_one(a.Y, a.y_type, i + x, o[x]);
                     }
                 }
                 __syncwarp();
@@ -431,8 +485,8 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
         ? make_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.W, (uint64_t)a.K, wrows, (uint64_t)p.ldw, C::BK, kTileC,
                       CU_TENSOR_MAP_SWIZZLE_128B)
         : make_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.W, (uint64_t)prepack_valid_words(a.K), wrows,
-                      (uint64_t)prepack_row_words(a.K, C::I8 ? 1 : 0) * 4, C::RAW_ROW ? C::RAW_ROW / 4 : 4, kTileC,
-                      CU_TENSOR_MAP_SWIZZLE_NONE);
+                      (uint64_t)prepack_row_words(a.K, C::I8 ? 1 : 0) * 4, C::DENSE ? 4 : C::RAW_PITCH / 4, kTileC,
+                      C::RAW_PITCH == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
     if (!okx || !okw) return TMQ_ERR_LAUNCH;
     int rc = ensure_dynamic_smem(scaled_gemm_kernel<WK, BN>, C::bytes(kMaxGroups));
     if (rc != TMQ_OK) return rc;
