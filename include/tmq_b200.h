@@ -266,7 +266,7 @@ int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *scale, int64_
  * (acc * row_scale) rounded, times scale plus bias in one fused multiply-add, rounded once more to y_type (TMQ_TYPE_*).
  * row_scale [M], scale [N], bias [N]: fp32, NULL for 1 / 1 / 0.  X int8 [M][ldx], 16-byte aligned, ldx % 16 == 0, any
  * K <= ldx (columns beyond K are not read).  Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw],
- * 16-byte aligned, ldw % 16 == 0.  Y [M][ldy], element-aligned (16-byte aligned with ldy % 8 == 0 takes vector stores).
+ * 16-byte aligned, ldw % 16 == 0.  Y [M][ldy], element-aligned.
  * *status: see "Status word" above.
  * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549, and the post_scale / bias of Linear.compact_forward, tmq/tmq.py:662-688. */
 int tmq_ternary_gemm_a8(const int8_t *X, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,

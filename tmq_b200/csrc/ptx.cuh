@@ -47,6 +47,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t parity) {
     return ok != 0;
 }
 
+// The same question without the hardware's own short wait
+__device__ __forceinline__ bool mbar_test_wait(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
 // Bounded wait: gives up after `budget` SM clock cycles (default ~2 s), or as soon as another CTA has flagged a failure,
 // records TMQ_ERR_TIMEOUT in *status and returns false.  Callers then skip their work and fall through to the teardown.
 constexpr long long kWaitBudgetCycles = 4000000000ll;

@@ -11,7 +11,7 @@
 //     (clamped to the rows that exist and made non-decreasing: bad boundaries give empty groups, never a bad address) and
 //     walks the units u = CTA, CTA + grid, ... through it.
 //   * Roles: warp 0 TMA of the activations (and 8-bit weights), warp 1 MMA issue, warp 2 TMA of the packed weights, then
-//     eight decode warps (packed weights only) and four epilogue warps.  Decoded
+//     decode warps (packed weights only) and epilogue warps.  Decoded
 //     weights go to tensor memory (the MMA reads its A operand there) except for int8 tiles of 256 rows, whose two
 //     accumulators fill tensor memory: those are decoded into shared memory.  8-bit weights need no decode, TMA writes
 //     them where the MMA reads them.
@@ -33,7 +33,6 @@ constexpr int kTileC = 128;          // channels of a unit (MMA M)
 constexpr int kOpRow = 128;          // bytes of one operand row per k-block: 64 bf16 or 128 int8
 constexpr int kRowStep = 32;         // granularity of a unit's MMA N
 constexpr int kMaxGroups = TMQ_GROUPS_MAX;
-constexpr int kDecodeWarps = 8;
 
 struct ScaledArgs {
     const float *row_scale;          // [M] or null (1)
@@ -57,8 +56,11 @@ struct ScaledCfg {
     static constexpr int RAWK = DENSE ? 1 : (TA ? 4 : 2);
     static constexpr int RAW_PITCH = RAWK * RAW_ROW;
     static constexpr int RAW_STAGES = DENSE ? 0 : !TA ? 2 : BN > 128 ? 2 : 4;
-    static constexpr int STAGES = DENSE ? (BN > 128 ? 4 : BN > 64 ? 6 : 8) : BN > 128 ? (TA ? 6 : 4) : 8;
-    static constexpr int A_BYTES = TA ? 0 : kTileC * kOpRow;
+    // A pipeline stage is KB k-blocks: the MMA warp pays its barrier round (about 270 cycles of latency) once a stage, and
+    // four MMAs of a k-block alone cover 170.  One k-block per stage measured 280 - 300 ns per k-block for every BN <= 128.
+    static constexpr int KB = !TA && BN > 128 ? 1 : (TA && BN <= 64) ? 4 : 2;
+    static constexpr int STAGES = DENSE ? (BN > 128 ? 4 : BN > 64 ? 3 : 4) : !TA ? 4 : BN > 128 ? 3 : BN > 64 ? 4 : 3;
+    static constexpr int A_BYTES = TA ? 0 : kTileC * kOpRow;                     // of one k-block
     static constexpr int B_BYTES = BN * kOpRow;
     static constexpr int RAW_BYTES = kTileC * RAW_PITCH;
     // activations arrive as one box of BN rows, or, for a unit of at most half of that, as one or two small boxes
@@ -66,18 +68,24 @@ struct ScaledCfg {
     static constexpr int ACC_BUFS = (TA && BN > 128) ? 1 : 2;
     static constexpr int A_COLS = kOpRow / 4;
     static constexpr int A_BASE = ACC_BUFS * BN;
-    static constexpr int TMEM_NEED = A_BASE + (TA ? STAGES * A_COLS : 0);
+    static constexpr int TMEM_NEED = A_BASE + (TA ? STAGES * KB * A_COLS : 0);
     static constexpr int TMEM_COLS = TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
     static_assert(TMEM_NEED <= 512, "tensor memory exceeded");
-    static constexpr int FIRST_EPI = DENSE ? 4 : 4 + kDecodeWarps;
-    static constexpr int THREADS = (FIRST_EPI + 4) * 32;
+    // Sets of four decode warps, one k-block of a stage each.  The integer pipe needs about 140 cycles for the codes of a
+    // k-block, a warp's round of waits and stores some 600 on top: tiles that do not hide that under their MMAs (four sets
+    // against two: 244 -> 185 ns per k-block of 64 rows) get four.
+    static constexpr int SETS = BN > 128 ? 2 : 4;
+    static constexpr int DECODERS = DENSE ? 0 : 4 * SETS;
+    static constexpr int FIRST_EPI = 4 + DECODERS;
+    static constexpr int EPI = BN > 128 ? 8 : 4;                              // epilogue warps
+    static constexpr int READY = 4 * KB;                                    // warps that decode one stage
+    static constexpr int THREADS = (FIRST_EPI + EPI) * 32;
     // shared memory
     static constexpr int A_OFF = 0;
-    static constexpr int B_OFF = A_OFF + STAGES * A_BYTES;
-    static constexpr int RAW_OFF = B_OFF + STAGES * B_BYTES;
-    static constexpr int STAGE_OFF = RAW_OFF + RAW_STAGES * RAW_BYTES;            // 4 x 2 KB transposition areas
-    static constexpr int RS_OFF = STAGE_OFF + 4 * 2048;                      // 4 x BN row scales
-    static constexpr int BAR_OFF = RS_OFF + 4 * BN * 4;
+    static constexpr int B_OFF = A_OFF + STAGES * KB * A_BYTES;
+    static constexpr int RAW_OFF = B_OFF + STAGES * KB * B_BYTES;
+    static constexpr int RS_OFF = RAW_OFF + RAW_STAGES * RAW_BYTES;           // 32 row scales per epilogue warp
+    static constexpr int BAR_OFF = RS_OFF + EPI * 128;
     static constexpr int TAB_OFF = BAR_OFF + 512;                             // begin[groups + 1], tiles[groups + 1]
     static constexpr int bytes(int groups) { return TAB_OFF + 2 * 4 * (groups + 1) + 1024; }
     static_assert(TAB_OFF + 2 * 4 * (kMaxGroups + 1) + 1024 <= 227 * 1024, "shared memory exceeded");
@@ -146,26 +154,49 @@ __device__ __forceinline__ void store_one(void *Y, int y_type, long long i, floa
     else reinterpret_cast<__half *>(Y)[i] = __float2half_rn(f);
 }
 
-// 8 consecutive channels of one row, aligned for vector stores
-__device__ __forceinline__ void store_eight(void *Y, int y_type, long long i, const float (&f)[8]) {
-    if (y_type == TMQ_TYPE_F32) {
-        float4 *p = reinterpret_cast<float4 *>(reinterpret_cast<float *>(Y) + i);
-        p[0] = make_float4(f[0], f[1], f[2], f[3]);
-        p[1] = make_float4(f[4], f[5], f[6], f[7]);
-        return;
-    }
-    uint32_t w[4];
+// One warp's 32 rows x 32 channels (f[j]: row j of this lane's channel) to Y.  TYPE fixed at compile time, addresses stepped.
+// FULL: all of them exist.  PAIRS: 16-bit results of two rows are paired between neighbouring lanes (even lanes keep row j,
+// odd lanes row j + 1), so a warp writes 4 bytes a lane, two 64-byte runs; otherwise one row's 32 channels at a time.
+template <int TYPE, bool PAIRS, bool FULL>
+__device__ __forceinline__ void store_rows(uint8_t *Y, long long row, long long ldy, int n, long long N, int left, int lane,
+                                           const float (&f)[32]) {
+    constexpr int ES = TYPE == TMQ_TYPE_F32 ? 4 : 2;
+    const int odd = PAIRS ? lane & 1 : 0;
+    const int nb = n - odd;
+    uint8_t *p = Y + ((row + odd) * ldy + nb) * ES;
+    const long long step = ldy * ES;
+    const int rows = nb < N ? left - odd : 0;
+    const bool both = nb + 1 < N;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (y_type == TMQ_TYPE_BF16) {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t *>(&h);
+    for (int j = 0; j < 32; j += (PAIRS ? 2 : 1)) {
+        if (PAIRS) {
+            const float got = __shfl_xor_sync(0xffffffffu, odd ? f[j] : f[j + (PAIRS ? 1 : 0)], 1);
+            const float lo = odd ? got : f[j], hi = odd ? f[j + (PAIRS ? 1 : 0)] : got;
+            uint32_t w;
+            if (TYPE == TMQ_TYPE_BF16) {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+                w = *reinterpret_cast<const uint32_t *>(&h);
+            } else {
+                const __half2 h = __floats2half2_rn(lo, hi);
+                w = *reinterpret_cast<const uint32_t *>(&h);
+            }
+            if (FULL || j < rows) {
+                if (FULL || both) *reinterpret_cast<uint32_t *>(p) = w;
+                else *reinterpret_cast<uint16_t *>(p) = (uint16_t)w;
+            }
+            p += 2 * step;
         } else {
-            const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t *>(&h);
+            if (FULL || j < rows) store_one(p, TYPE, 0, f[j]);
+            p += step;
         }
     }
-    *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(Y) + i) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <int TYPE, bool PAIRS>
+__device__ __forceinline__ void store_rows(uint8_t *Y, long long row, long long ldy, int n, long long N, int left, int lane,
+                                           const float (&f)[32]) {
+    if (left >= 32 && n - lane + 32 <= N) store_rows<TYPE, PAIRS, true>(Y, row, ldy, n, N, left, lane, f);
+    else store_rows<TYPE, PAIRS, false>(Y, row, ldy, n, N, left, lane, f);
 }
 
 template <int WK, int BN>
@@ -194,16 +225,16 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::STAGES; s++) {
             ptx::mbar_init(full + s, 1);
-            ptx::mbar_init(ready + s, 4);
+            ptx::mbar_init(ready + s, C::READY);
             ptx::mbar_init(empty + s, 1);
         }
         for (int s = 0; s < C::RAW_STAGES; s++) {
             ptx::mbar_init(raw_full + s, 1);
-            ptx::mbar_init(raw_empty + s, kDecodeWarps);
+            ptx::mbar_init(raw_empty + s, C::DECODERS);
         }
         for (int b = 0; b < 2; b++) {
             ptx::mbar_init(acc_full + b, 1);
-            ptx::mbar_init(acc_empty + b, 4);
+            ptx::mbar_init(acc_empty + b, C::EPI);
         }
         ptx::fence_mbar_init();
         ptx::prefetch_tensormap(&tmap_x);
@@ -233,18 +264,21 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                 const bool whole = q.rows > BN / 2;
                 const int rows = whole ? BN : q.rows > C::SMALL ? 2 * C::SMALL : C::SMALL;
                 const int wrow = (int)(q.e * a.N) + q.n0;
-                const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : 0));
-                for (int kb = 0; kb < nkb; kb++, it++) {
-                    const int s = it % C::STAGES;
+                const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : 0));      // of one k-block
+                for (int kb = 0; kb < nkb; kb += C::KB, it++) {
+                    const int s = it % C::STAGES, n = nkb - kb < C::KB ? nkb - kb : C::KB;
                     const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
                     ok = ptx::mbar_wait(empty + s, ph ^ 1u, a.status);
                     if (!ok) break;
-                    ptx::mbar_arrive_expect_tx(full + s, bytes);
-                    if (C::DENSE) ptx::tma_load_2d(smem + C::A_OFF + s * C::A_BYTES, &tmap_w, full + s, kb * C::BK, wrow);
-                    uint8_t *dst = smem + C::B_OFF + s * C::B_BYTES;
-                    ptx::tma_load_2d(dst, whole ? &tmap_x : &tmap_small, full + s, kb * C::BK, q.row0);
-                    if (!whole && rows > C::SMALL)
-                        ptx::tma_load_2d(dst + C::SMALL * kOpRow, &tmap_small, full + s, kb * C::BK, q.row0 + C::SMALL);
+                    ptx::mbar_arrive_expect_tx(full + s, bytes * (uint32_t)n);
+                    for (int j = 0; j < n; j++) {
+                        const int x = (kb + j) * C::BK;
+                        if (C::DENSE) ptx::tma_load_2d(smem + C::A_OFF + (s * C::KB + j) * C::A_BYTES, &tmap_w, full + s, x, wrow);
+                        uint8_t *dst = smem + C::B_OFF + (s * C::KB + j) * C::B_BYTES;
+                        ptx::tma_load_2d(dst, whole ? &tmap_x : &tmap_small, full + s, x, q.row0);
+                        if (!whole && rows > C::SMALL)
+                            ptx::tma_load_2d(dst + C::SMALL * kOpRow, &tmap_small, full + s, x, q.row0 + C::SMALL);
+                    }
                 }
             }
         }
@@ -252,7 +286,9 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
         // ---------------------------------------------------------------- MMA issuer (whole warp walks, one lane issues)
         if (healthy) {
             int it = 0, ti = 0, e = 0;
-            bool ok = true;
+            bool ok = true, landed = false;
+            // even lanes watch the weights' barrier, odd lanes the activations': one round for both
+            uint64_t *const watch = (C::DENSE || (lane & 1)) ? full : ready;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x, ti++) {
                 const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
                 const uint32_t n_mma = (uint32_t)((q.rows + kRowStep - 1) / kRowStep * kRowStep);
@@ -263,31 +299,36 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(buf * BN);
-                for (int kb = 0; kb < nkb; kb++, it++) {
+                for (int kb = 0; kb < nkb; kb += C::KB, it++) {
                     const int s = it % C::STAGES;
-                    const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
-                    if (!C::DENSE) ok = ptx::mbar_wait_warp(ready + s, ph, a.status);
-                    // the activations were written by TMA: their barrier is waited on by this warp itself
-                    ok = ok && ptx::mbar_wait_warp(full + s, ph, a.status);
+                    if (!landed) ok = ptx::mbar_wait_warp(watch + s, (uint32_t)(it / C::STAGES) & 1u, a.status);
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
-                    const uint64_t a_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::A_OFF + s * C::A_BYTES));
-                    const uint64_t b_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::B_OFF + s * C::B_BYTES));
-                    const uint32_t a_tmem = tmem_base + C::A_BASE + (uint32_t)(s * C::A_COLS);
+                    // the next stage is looked up while this one's MMAs are issued
+                    const bool next = ptx::mbar_test_wait(watch + (it + 1) % C::STAGES, (uint32_t)((it + 1) / C::STAGES) & 1u);
+                    const uint64_t a_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::A_OFF + s * C::KB * C::A_BYTES));
+                    const uint64_t b_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::B_OFF + s * C::KB * C::B_BYTES));
+                    const uint32_t a_tmem = tmem_base + C::A_BASE + (uint32_t)(s * C::KB * C::A_COLS);
                     if (ptx::elect_one()) {
 #pragma unroll
-                        for (int k4 = 0; k4 < kOpRow / 32; k4++) {
-                            const uint32_t accum = (kb > 0 || k4 > 0) ? 1u : 0u;
-                            if (C::TA) {
-                                if (C::I8) ptx::umma_i8_ts(d_tmem, a_tmem + 8 * k4, b_desc + 2 * k4, idesc, accum);
-                                else ptx::umma_f16_ts(d_tmem, a_tmem + 8 * k4, b_desc + 2 * k4, idesc, accum);
-                            } else {
-                                ptx::umma_i8(d_tmem, a_desc + 2 * k4, b_desc + 2 * k4, idesc, accum);
+                        for (int j = 0; j < C::KB; j++) {
+                            if (j > 0 && kb + j >= nkb) break;
+#pragma unroll
+                            for (int k4 = 0; k4 < kOpRow / 32; k4++) {
+                                const uint32_t accum = (kb > 0 || j > 0 || k4 > 0) ? 1u : 0u;
+                                const uint64_t bd = b_desc + (uint64_t)(j * (C::B_BYTES >> 4) + 2 * k4);
+                                if (C::TA) {
+                                    const uint32_t at = a_tmem + (uint32_t)(j * C::A_COLS + 8 * k4);
+                                    if (C::I8) ptx::umma_i8_ts(d_tmem, at, bd, idesc, accum);
+                                    else ptx::umma_f16_ts(d_tmem, at, bd, idesc, accum);
+                                } else {
+                                    ptx::umma_i8(d_tmem, a_desc + (uint64_t)(j * (C::A_BYTES >> 4) + 2 * k4), bd, idesc, accum);
+                                }
                             }
                         }
                         ptx::umma_commit(empty + s);
                     }
-                    __syncwarp();
+                    landed = __all_sync(0xffffffffu, next ? 1 : 0) != 0;
                 }
                 if (ok && ptx::elect_one()) ptx::umma_commit(acc_full + buf);
                 __syncwarp();
@@ -312,77 +353,89 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             }
         }
     } else if (!C::DENSE && warp >= 4 && warp < C::FIRST_EPI) {
-        // ---------------------------------------------------------------- decode: two sets of four warps, alternate k-blocks
+        // ---------------------------------------------------------------- decode
         const int quarter = warp & 3, set = (warp - 4) >> 2;
         const int row = quarter * 32 + lane;
         bool ok = healthy;
-        int it = 0, rit = 0;
+        int it = 0, s = 0, rs = 0;
+        uint32_t ph = 0, rph = 0;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            for (int kb0 = 0; kb0 < nkb && ok; kb0 += C::RAWK, rit++) {
-                const int rs = rit % (C::RAW_STAGES + C::DENSE);
-                ok = ptx::mbar_wait_warp(raw_full + rs, (uint32_t)(rit / (C::RAW_STAGES + C::DENSE)) & 1u, a.status);
-                if (!ok) break;
+            for (int kb0 = 0; kb0 < nkb && ok; kb0 += C::RAWK) {
                 const uint8_t *raw = smem + C::RAW_OFF + rs * C::RAW_BYTES + row * C::RAW_PITCH;
-                const int left = nkb - kb0 < C::RAWK ? nkb - kb0 : C::RAWK;
-                for (int j = (it & 1) ^ set; j < left; j += 2) {
-                    const int s = (it + j) % C::STAGES;
-                    const uint32_t ph = (uint32_t)((it + j) / C::STAGES) & 1u;
-                    uint4 p[C::I8 ? 2 : 1];
-#pragma unroll
-                    for (int h = 0; h < (C::I8 ? 2 : 1); h++) {
-                        const int c = (C::I8 ? 2 * j : j) + h;
-                        p[h] = *reinterpret_cast<const uint4 *>(raw + ((c ^ (C::RAW_PITCH == 128 ? row & 7 : (row >> 1) & 3)) << 4));
-                    }
-                    uint32_t cols[32];                   // the row's 128 operand bytes, K ascending
-                    if (C::I8) {
-                        const uint32_t words[8] = {p[0].x, p[0].y, p[0].z, p[0].w, p[C::I8].x, p[C::I8].y, p[C::I8].z, p[C::I8].w};
-#pragma unroll
-                        for (int wi = 0; wi < 8; wi++) {
-                            uint32_t r[4];
-                            decode_word_i8(words[wi], r);
-#pragma unroll
-                            for (int x = 0; x < 4; x++) cols[4 * wi + x] = r[x];
-                        }
-                    } else {
-                        const uint32_t words[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
-#pragma unroll
-                        for (int wi = 0; wi < 4; wi++) {
-                            uint32_t r[8];
-                            decode_word_bf16(words[wi], r);
-#pragma unroll
-                            for (int x = 0; x < 8; x++) cols[8 * wi + x] = r[x];
-                        }
-                    }
-                    // the MMAs that read this operand slot last are done
-                    ok = ptx::mbar_wait_warp(empty + s, ph ^ 1u, a.status);
+                bool seen = false;
+                for (int st = 0; st < C::RAWK && kb0 + st < nkb; st += C::KB) {
+                    // k-block j of stage it belongs to set (it KB + j) mod SETS
+                    const int j = (set - it * C::KB) & (C::SETS - 1);
+                    if (j < C::KB) {
+                    // even lanes wait for the packed words, odd lanes until the MMAs that read this stage last are done; a
+                    // set whose k-block lies beyond the unit waits (and reports) as well, or it would run a round ahead
+                    ok = ptx::mbar_wait_warp((lane & 1) ? empty + s : raw_full + rs, (lane & 1) ? ph ^ 1u : rph, a.status);
                     if (!ok) break;
+                    seen = true;
+                    if (kb0 + st + j < nkb) {
+                        uint4 p[C::I8 ? 2 : 1];
+#pragma unroll
+                        for (int h = 0; h < (C::I8 ? 2 : 1); h++) {
+                            const int c = (C::I8 ? 2 * (st + j) : st + j) + h;
+                            p[h] = *reinterpret_cast<const uint4 *>(raw + ((c ^ (C::RAW_PITCH == 128 ? row & 7 : (row >> 1) & 3)) << 4));
+                        }
+                        uint32_t cols[32];                   // the row's 128 operand bytes, K ascending
+                        if (C::I8) {
+                            const uint32_t words[8] = {p[0].x, p[0].y, p[0].z, p[0].w, p[C::I8].x, p[C::I8].y, p[C::I8].z, p[C::I8].w};
+#pragma unroll
+                            for (int wi = 0; wi < 8; wi++) {
+                                uint32_t r[4];
+                                decode_word_i8_ptx(words[wi], r);
+#pragma unroll
+                                for (int x = 0; x < 4; x++) cols[4 * wi + x] = r[x];
+                            }
+                        } else {
+                            const uint32_t words[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
+#pragma unroll
+                            for (int wi = 0; wi < 4; wi++) {
+                                uint32_t r[8];
+                                decode_word_bf16(words[wi], r);
+#pragma unroll
+                                for (int x = 0; x < 8; x++) cols[8 * wi + x] = r[x];
+                            }
+                        }
+                        if (C::TA) {
+                            ptx::tc_fence_after_sync();
+                            ptx::tmem_st_x32(tmem_base + ((uint32_t)(quarter * 32) << 16) + C::A_BASE +
+                                                 (uint32_t)((s * C::KB + j) * C::A_COLS), cols);
+                        } else {
+                            uint8_t *arow = smem + C::A_OFF + (s * C::KB + j) * C::A_BYTES + row * kOpRow;
+#pragma unroll
+                            for (int c = 0; c < 8; c++)
+                                *reinterpret_cast<uint4 *>(arow + ((c ^ (row & 7)) << 4)) =
+                                    make_uint4(cols[4 * c], cols[4 * c + 1], cols[4 * c + 2], cols[4 * c + 3]);
+                        }
+                    }
                     if (C::TA) {
-                        ptx::tc_fence_after_sync();
-                        ptx::tmem_st_x32(tmem_base + ((uint32_t)(quarter * 32) << 16) + C::A_BASE + (uint32_t)(s * C::A_COLS), cols);
                         ptx::tmem_st_wait();
                         ptx::tc_fence_before_sync();
                     } else {
-                        uint8_t *arow = smem + C::A_OFF + s * C::A_BYTES + row * kOpRow;
-#pragma unroll
-                        for (int c = 0; c < 8; c++)
-                            *reinterpret_cast<uint4 *>(arow + ((c ^ (row & 7)) << 4)) =
-                                make_uint4(cols[4 * c], cols[4 * c + 1], cols[4 * c + 2], cols[4 * c + 3]);
                         ptx::fence_proxy_async_smem();
                     }
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(ready + s);
+                    }
+                    it++;
+                    if (++s == C::STAGES) { s = 0; ph ^= 1u; }
                 }
-                it += left;
+                if (ok && !seen) ok = ptx::mbar_wait_warp(raw_full + rs, rph, a.status);
                 __syncwarp();
                 if (ok && lane == 0) ptx::mbar_arrive(raw_empty + rs);
+                if (++rs == C::RAW_STAGES + C::DENSE) { rs = 0; rph ^= 1u; }
             }
         }
     } else if (warp >= C::FIRST_EPI) {
         // ---------------------------------------------------------------- epilogue
-        const int quarter = warp & 3;
-        float *stage = reinterpret_cast<float *>(smem + C::STAGE_OFF) + (warp - C::FIRST_EPI) * 512;
-        float *rs = reinterpret_cast<float *>(smem + C::RS_OFF) + (warp - C::FIRST_EPI) * BN;
-        const bool vec_rows = ((a.ldy & 7) == 0) && ((reinterpret_cast<uintptr_t>(a.Y) & 15) == 0);
+        // lane = channel, accumulator column = row: 32 rows at a time
+        const int quarter = warp & 3, group = (warp - C::FIRST_EPI) >> 2;
+        constexpr int kStep = 8 * C::EPI;                 // rows the epilogue warps of a quarter take per round
+        float *rs = reinterpret_cast<float *>(smem + C::RS_OFF) + (warp - C::FIRST_EPI) * 32;
+        const bool pairs = a.y_type != TMQ_TYPE_F32 && (a.ldy & 1) == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 3) == 0;
         bool ok = healthy;
         int ti = 0, e = 0;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x, ti++) {
@@ -394,56 +447,45 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                 if (a.bias) bi = a.bias[(long long)q.e * a.N + n];
             }
             if (!C::I8) sc *= 0.5f;                      // bf16 weights are carried as +-2
-            __syncwarp();
-            for (int r = lane; r < BN; r += 32) rs[r] = (a.row_scale && r < q.rows) ? a.row_scale[q.row0 + r] : 1.0f;
-            __syncwarp();
             const int buf = C::ACC_BUFS == 2 ? (ti & 1) : 0;
             ok = ptx::mbar_wait_warp(acc_full + buf, (uint32_t)(C::ACC_BUFS == 2 ? (ti >> 1) : ti) & 1u, a.status);
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN);
 #pragma unroll 1
-            for (int c = 0; c < q.rows; c += 16) {
-                uint32_t v[16];
-                ptx::tmem_ld_x16(lane_addr + (uint32_t)c, v);
-                ptx::tmem_ld_wait();
-                if (c + 16 >= q.rows) {                  // last chunk read: the accumulator goes back to the MMA warp
+            for (int c = 32 * group; c < q.rows + kStep; c += kStep) {
+                if (c >= q.rows) {                       // nothing (more) to read: the accumulator goes back to the MMA warp
                     ptx::tc_fence_before_sync();
                     __syncwarp();
                     if (lane == 0) ptx::mbar_arrive(acc_empty + buf);
+                    break;
                 }
-                float f[16];
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    const float acc = C::I8 ? __int2float_rn((int)v[j]) : __uint_as_float(v[j]);
-                    f[j] = fmaf(__fmul_rn(acc, rs[c + j]), sc, bi);
+                uint32_t v[32];
+                ptx::tmem_ld_x16(lane_addr + (uint32_t)c, reinterpret_cast<uint32_t(&)[16]>(v[0]));
+                ptx::tmem_ld_x16(lane_addr + (uint32_t)c + 16, reinterpret_cast<uint32_t(&)[16]>(v[16]));
+                if (C::I8) {
+                    const float r = (a.row_scale && c + lane < q.rows) ? a.row_scale[q.row0 + c + lane] : 1.0f;
+                    __syncwarp();
+                    rs[lane] = r;
+                    __syncwarp();
                 }
-                if (!vec_rows) {                         // rows that allow no vectors: a warp writes 32 neighbouring channels
-                    if (n < a.N) {
+                ptx::tmem_ld_wait();
+                const int left = q.rows - c;
+                float f[32];
 #pragma unroll
-                        for (int j = 0; j < 16; j++)
-                            if (c + j < q.rows) store_one(a.Y, a.y_type, (long long)(q.row0 + c + j) * a.ldy + n, f[j]);
-                    }
-                    continue;
+                for (int j = 0; j < 32; j++) {
+                    const float acc = C::I8 ? __fmul_rn(__int2float_rn((int)v[j]), rs[j]) : __uint_as_float(v[j]);
+                    f[j] = fmaf(acc, sc, bi);
                 }
-#pragma unroll
-                for (int j = 0; j < 16; j++) stage[j * 32 + lane] = f[j];
-                __syncwarp();
-                const int cg = (lane & 3) * 8, nb = q.n0 + quarter * 32 + cg;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const int p = h * 8 + (lane >> 2);
-                    if (c + p < q.rows && nb < a.N) {
-                        const float4 lo = *reinterpret_cast<const float4 *>(stage + p * 32 + cg);
-                        const float4 hi = *reinterpret_cast<const float4 *>(stage + p * 32 + cg + 4);
-                        const float o[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-                        const long long i = (long long)(q.row0 + c + p) * a.ldy + nb;
-                        if (nb + 8 <= a.N) store_eight(a.Y, a.y_type, i, o);
-                        else
-                            for (int x = 0; x < 8 && nb + x < a.N; x++) store_one(a.Y, a.y_type, i + x, o[x]);
-                    }
-                }
-                __syncwarp();
+                uint8_t *Y = reinterpret_cast<uint8_t *>(a.Y);
+                const long long row = q.row0 + c;
+                if (a.y_type == TMQ_TYPE_F32) store_rows<TMQ_TYPE_F32, false>(Y, row, a.ldy, n, a.N, left, lane, f);
+                else if (a.y_type == TMQ_TYPE_BF16)
+                    pairs ? store_rows<TMQ_TYPE_BF16, true>(Y, row, a.ldy, n, a.N, left, lane, f)
+                          : store_rows<TMQ_TYPE_BF16, false>(Y, row, a.ldy, n, a.N, left, lane, f);
+                else
+                    pairs ? store_rows<TMQ_TYPE_F16, true>(Y, row, a.ldy, n, a.N, left, lane, f)
+                          : store_rows<TMQ_TYPE_F16, false>(Y, row, a.ldy, n, a.N, left, lane, f);
             }
         }
         if (a.zero_rest && healthy) {
@@ -451,7 +493,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             const long long lead = begin[0], tail = begin[a.groups], total = lead + (a.M - tail);
             for (long long r = blockIdx.x; r < total; r += gridDim.x) {
                 const long long m = r < lead ? r : tail + (r - lead);
-                for (long long n = threadIdx.x - C::FIRST_EPI * 32; n < a.N; n += 128) store_one(a.Y, a.y_type, m * a.ldy + n, 0.0f);
+                for (long long n = threadIdx.x - C::FIRST_EPI * 32; n < a.N; n += C::EPI * 32)
+                    store_one(a.Y, a.y_type, m * a.ldy + n, 0.0f);
             }
         }
     }
