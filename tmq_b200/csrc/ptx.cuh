@@ -79,7 +79,30 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, int *s
     }
 }
 
-// The same wait made by a whole converged warp, with a warp-uniform result (one lane giving up makes every lane give up),
+// The same wait for a thread that expects to wait long (a copy producer, an epilogue): the hardware may hold each try for up
+// to 20 us, which leaves the issue slots of its scheduler to the warps that compute.
+__device__ __forceinline__ bool mbar_wait_idle(uint64_t *bar, uint32_t parity, int *status,
+                                               long long budget = kWaitBudgetCycles) {
+    const long long t0 = clock64();
+    for (;;) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+            : "memory");
+        if (ok) return true;
+        if (*reinterpret_cast<volatile int *>(status) != 0) return false;
+        if (clock64() - t0 > budget) {
+            atomicCAS(status, 0, TMQ_ERR_TIMEOUT);
+            return false;
+        }
+    }
+}
+
+// mbar_wait made by a whole converged warp, with a warp-uniform result (one lane giving up makes every lane give up),
 // so that code after it can stay convergent (elect_one needs the full warp).
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, int *status,
                                                long long budget = kWaitBudgetCycles) {
@@ -100,6 +123,13 @@ __device__ __forceinline__ void tma_load_2d(void *smem_dst, const CUtensorMap *m
     asm volatile(
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *map, uint64_t *bar, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+        ::"r"(smem_u32(smem_dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
         : "memory");
 }
 

@@ -34,6 +34,12 @@ constexpr int kOpRow = 128;          // bytes of one operand row per k-block: 64
 constexpr int kRowStep = 32;         // granularity of a unit's MMA N
 constexpr int kMaxGroups = TMQ_GROUPS_MAX;
 
+// Tensor maps of a launch.  A TMA instruction costs about 200 cycles of its unit whatever it brings (bf16 tiles of 32 rows
+// with one box per k-block: 154 ns per k-block), so a box spans all k-blocks of a stage where the row length allows it.
+struct ScaledMaps {
+    CUtensorMap x[3], w;
+};
+
 struct ScaledArgs {
     const float *row_scale;          // [M] or null (1)
     const float *scale, *bias;       // [groups][N] or null (1 / 0)
@@ -41,6 +47,7 @@ struct ScaledArgs {
     const void *offsets;             // [groups + 1] int32 or int64, null: one group of all rows
     long long M, N, K, ldy;
     int groups, offsets64, y_type, zero_rest;
+    int wide;                        // K is whole k-blocks: one box per stage
     int *status;
 };
 
@@ -55,20 +62,25 @@ struct ScaledCfg {
     // width, so the decode warps' 16-byte reads meet no bank conflicts.
     static constexpr int RAWK = DENSE ? 1 : (TA ? 4 : 2);
     static constexpr int RAW_PITCH = RAWK * RAW_ROW;
-    static constexpr int RAW_STAGES = DENSE ? 0 : !TA ? 2 : BN > 128 ? 2 : 4;
     // A pipeline stage is KB k-blocks: the MMA warp pays its barrier round (about 270 cycles of latency) once a stage, and
     // four MMAs of a k-block alone cover 170.  One k-block per stage measured 280 - 300 ns per k-block for every BN <= 128.
     static constexpr int KB = !TA && BN > 128 ? 1 : (TA && BN <= 64) ? 4 : 2;
-    static constexpr int STAGES = DENSE ? (BN > 128 ? 4 : BN > 64 ? 3 : 4) : !TA ? 4 : BN > 128 ? 3 : BN > 64 ? 4 : 3;
+    // Three rings: decoded weights (NA stages; tensor memory, or shared memory for int8 tiles of 256 rows), activations and
+    // 8-bit weights (NB stages), packed words (RAW_STAGES boxes).  An activation box takes about 1250 cycles from L2, so its
+    // ring is the one that must be deep: three stages of four k-blocks, shared with the weights, held bf16 tiles of 64 rows
+    // at 154 ns per k-block.
+    static constexpr int NA = DENSE ? 0 : !TA ? 4 : BN > 128 ? 3 : BN > 64 ? 4 : 3;
+    static constexpr int NB = DENSE ? (BN > 128 ? 4 : BN > 64 ? 3 : BN > 32 ? 4 : 5) : !TA ? 4 : BN > 128 ? 3 : BN > 64 ? 5 : BN > 32 ? 4 : 7;
+    static constexpr int RAW_STAGES = DENSE ? 0 : !TA ? 2 : BN > 128 ? 2 : BN > 64 ? 3 : 4;
     static constexpr int A_BYTES = TA ? 0 : kTileC * kOpRow;                     // of one k-block
     static constexpr int B_BYTES = BN * kOpRow;
     static constexpr int RAW_BYTES = kTileC * RAW_PITCH;
-    // activations arrive as one box of BN rows, or, for a unit of at most half of that, as one or two small boxes
-    static constexpr int SMALL = BN > 128 ? 64 : 32;
+    // heights of the activation boxes: a unit takes the lowest that holds its rows
+    static constexpr int BOX0 = BN, BOX1 = BN > 32 ? BN / 2 : 32, BOX2 = BN > 64 ? BN / 4 : 32;
     static constexpr int ACC_BUFS = (TA && BN > 128) ? 1 : 2;
     static constexpr int A_COLS = kOpRow / 4;
     static constexpr int A_BASE = ACC_BUFS * BN;
-    static constexpr int TMEM_NEED = A_BASE + (TA ? STAGES * KB * A_COLS : 0);
+    static constexpr int TMEM_NEED = A_BASE + (TA ? NA * KB * A_COLS : 0);
     static constexpr int TMEM_COLS = TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
     static_assert(TMEM_NEED <= 512, "tensor memory exceeded");
     // Sets of four decode warps, one k-block of a stage each.  The integer pipe needs about 140 cycles for the codes of a
@@ -82,8 +94,8 @@ struct ScaledCfg {
     static constexpr int THREADS = (FIRST_EPI + EPI) * 32;
     // shared memory
     static constexpr int A_OFF = 0;
-    static constexpr int B_OFF = A_OFF + STAGES * KB * A_BYTES;
-    static constexpr int RAW_OFF = B_OFF + STAGES * KB * B_BYTES;
+    static constexpr int B_OFF = A_OFF + (DENSE ? NB : NA) * KB * A_BYTES;
+    static constexpr int RAW_OFF = B_OFF + NB * KB * B_BYTES;
     static constexpr int RS_OFF = RAW_OFF + RAW_STAGES * RAW_BYTES;           // 32 row scales per epilogue warp
     static constexpr int BAR_OFF = RS_OFF + EPI * 128;
     static constexpr int TAB_OFF = BAR_OFF + 512;                             // begin[groups + 1], tiles[groups + 1]
@@ -201,15 +213,15 @@ __device__ __forceinline__ void store_rows(uint8_t *Y, long long row, long long 
 
 template <int WK, int BN>
 __global__ void __launch_bounds__(ScaledCfg<WK, BN>::THREADS, 1)
-scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_small,
-                   const __grid_constant__ CUtensorMap tmap_w, const ScaledArgs a) {
+scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) {
     using C = ScaledCfg<WK, BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);         // TMA bytes landed
-    uint64_t *ready = full + C::STAGES;                                       // weights decoded
-    uint64_t *empty = ready + C::STAGES;
-    uint64_t *raw_full = empty + C::STAGES;                                   // packed words landed
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BAR_OFF);         // activations (and 8-bit weights) landed
+    uint64_t *empty = full + C::NB;
+    uint64_t *ready = empty + C::NB;                                          // weights decoded
+    uint64_t *taken = ready + C::NA;                                          // ... and multiplied
+    uint64_t *raw_full = taken + C::NA;                                   // packed words landed
     uint64_t *raw_empty = raw_full + C::RAW_STAGES;
     uint64_t *acc_full = raw_empty + C::RAW_STAGES;                           // [2]
     uint64_t *acc_empty = acc_full + 2;                                       // [2]
@@ -223,10 +235,13 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
-        for (int s = 0; s < C::STAGES; s++) {
+        for (int s = 0; s < C::NB; s++) {
             ptx::mbar_init(full + s, 1);
-            ptx::mbar_init(ready + s, C::READY);
             ptx::mbar_init(empty + s, 1);
+        }
+        for (int s = 0; s < C::NA; s++) {
+            ptx::mbar_init(ready + s, C::READY);
+            ptx::mbar_init(taken + s, 1);
         }
         for (int s = 0; s < C::RAW_STAGES; s++) {
             ptx::mbar_init(raw_full + s, 1);
@@ -237,9 +252,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             ptx::mbar_init(acc_empty + b, C::EPI);
         }
         ptx::fence_mbar_init();
-        ptx::prefetch_tensormap(&tmap_x);
-        ptx::prefetch_tensormap(&tmap_small);
-        ptx::prefetch_tensormap(&tmap_w);
+        for (int i = 0; i < 3; i++) ptx::prefetch_tensormap(maps.x + i);
+        ptx::prefetch_tensormap(&maps.w);
     }
     if (warp == 1) {
         ptx::tmem_alloc(tmem_slot, C::TMEM_COLS);
@@ -257,41 +271,46 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
         if (lane == 0 && healthy) {
-            int it = 0, e = 0;
+            int s = 0, e = 0;
+            uint32_t ph = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
                 const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
-                const bool whole = q.rows > BN / 2;
-                const int rows = whole ? BN : q.rows > C::SMALL ? 2 * C::SMALL : C::SMALL;
+                const int rows = q.rows > C::BOX1 ? C::BOX0 : q.rows > C::BOX2 ? C::BOX1 : C::BOX2;
+                const CUtensorMap *mx = maps.x + (q.rows > C::BOX1 ? 0 : q.rows > C::BOX2 ? 1 : 2);
                 const int wrow = (int)(q.e * a.N) + q.n0;
                 const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : 0));      // of one k-block
-                for (int kb = 0; kb < nkb; kb += C::KB, it++) {
-                    const int s = it % C::STAGES, n = nkb - kb < C::KB ? nkb - kb : C::KB;
-                    const uint32_t ph = (uint32_t)(it / C::STAGES) & 1u;
-                    ok = ptx::mbar_wait(empty + s, ph ^ 1u, a.status);
+                for (int kb = 0; kb < nkb; kb += C::KB) {
+                    const int n = nkb - kb < C::KB ? nkb - kb : C::KB;
+                    ok = ptx::mbar_wait_idle(empty + s, ph, a.status);
                     if (!ok) break;
-                    ptx::mbar_arrive_expect_tx(full + s, bytes * (uint32_t)n);
-                    for (int j = 0; j < n; j++) {
-                        const int x = (kb + j) * C::BK;
-                        if (C::DENSE) ptx::tma_load_2d(smem + C::A_OFF + (s * C::KB + j) * C::A_BYTES, &tmap_w, full + s, x, wrow);
-                        uint8_t *dst = smem + C::B_OFF + (s * C::KB + j) * C::B_BYTES;
-                        ptx::tma_load_2d(dst, whole ? &tmap_x : &tmap_small, full + s, x, q.row0);
-                        if (!whole && rows > C::SMALL)
-                            ptx::tma_load_2d(dst + C::SMALL * kOpRow, &tmap_small, full + s, x, q.row0 + C::SMALL);
+                    uint8_t *wd = smem + C::A_OFF + s * C::KB * C::A_BYTES, *xd = smem + C::B_OFF + s * C::KB * C::B_BYTES;
+                    ptx::mbar_arrive_expect_tx(full + s, bytes * (uint32_t)(a.wide ? C::KB : n));
+                    if (a.wide) {                        // k-blocks beyond the row are filled with zeros, and counted
+                        if (C::DENSE) ptx::tma_load_3d(wd, &maps.w, full + s, 0, wrow, kb);
+                        ptx::tma_load_3d(xd, mx, full + s, 0, q.row0, kb);
+                    } else {
+                        for (int j = 0; j < n; j++) {
+                            if (C::DENSE) ptx::tma_load_3d(wd + j * C::A_BYTES, &maps.w, full + s, (kb + j) * C::BK, wrow, 0);
+                            ptx::tma_load_3d(xd + j * rows * kOpRow, mx, full + s, (kb + j) * C::BK, q.row0, 0);
+                        }
                     }
+                    if (++s == C::NB) { s = 0; ph ^= 1u; }
                 }
             }
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (whole warp walks, one lane issues)
         if (healthy) {
-            int it = 0, ti = 0, e = 0;
+            int sa = 0, sb = 0, ti = 0, e = 0;
+            uint32_t pa = 0, pb = 0;
             bool ok = true, landed = false;
             // even lanes watch the weights' barrier, odd lanes the activations': one round for both
-            uint64_t *const watch = (C::DENSE || (lane & 1)) ? full : ready;
+            const bool acts = C::DENSE || (lane & 1);
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x, ti++) {
                 const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
                 const uint32_t n_mma = (uint32_t)((q.rows + kRowStep - 1) / kRowStep * kRowStep);
+                const uint32_t b_step = (uint32_t)((q.rows > C::BOX1 ? C::BOX0 : q.rows > C::BOX2 ? C::BOX1 : C::BOX2) * kOpRow) >> 4;
                 const uint32_t idesc = ((C::I8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((n_mma >> 3) << 17) | ((128u >> 4) << 24);
                 const int buf = C::ACC_BUFS == 2 ? (ti & 1) : 0;
                 const uint32_t use = (uint32_t)(C::ACC_BUFS == 2 ? (ti >> 1) : ti);
@@ -299,16 +318,18 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                 if (!ok) break;
                 ptx::tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(buf * BN);
-                for (int kb = 0; kb < nkb; kb += C::KB, it++) {
-                    const int s = it % C::STAGES;
-                    if (!landed) ok = ptx::mbar_wait_warp(watch + s, (uint32_t)(it / C::STAGES) & 1u, a.status);
+                for (int kb = 0; kb < nkb; kb += C::KB) {
+                    if (!landed) ok = ptx::mbar_wait_warp(acts ? full + sb : ready + sa, acts ? pb : pa, a.status);
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
+                    const uint64_t a_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::A_OFF + (C::DENSE ? sb : sa) * C::KB * C::A_BYTES));
+                    const uint64_t b_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::B_OFF + sb * C::KB * C::B_BYTES));
+                    const uint32_t a_tmem = tmem_base + C::A_BASE + (uint32_t)(sa * C::KB * C::A_COLS);
+                    uint64_t *const used_a = taken + sa, *const used_b = empty + sb;
+                    if (++sb == C::NB) { sb = 0; pb ^= 1u; }
+                    if (++sa >= C::NA) { sa = 0; pa ^= 1u; }
                     // the next stage is looked up while this one's MMAs are issued
-                    const bool next = ptx::mbar_test_wait(watch + (it + 1) % C::STAGES, (uint32_t)((it + 1) / C::STAGES) & 1u);
-                    const uint64_t a_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::A_OFF + s * C::KB * C::A_BYTES));
-                    const uint64_t b_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::B_OFF + s * C::KB * C::B_BYTES));
-                    const uint32_t a_tmem = tmem_base + C::A_BASE + (uint32_t)(s * C::KB * C::A_COLS);
+                    const bool next = ptx::mbar_test_wait(acts ? full + sb : ready + sa, acts ? pb : pa);
                     if (ptx::elect_one()) {
 #pragma unroll
                         for (int j = 0; j < C::KB; j++) {
@@ -316,7 +337,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
 #pragma unroll
                             for (int k4 = 0; k4 < kOpRow / 32; k4++) {
                                 const uint32_t accum = (kb > 0 || j > 0 || k4 > 0) ? 1u : 0u;
-                                const uint64_t bd = b_desc + (uint64_t)(j * (C::B_BYTES >> 4) + 2 * k4);
+                                const uint64_t bd = b_desc + (uint64_t)(j * b_step + 2 * k4);
                                 if (C::TA) {
                                     const uint32_t at = a_tmem + (uint32_t)(j * C::A_COLS + 8 * k4);
                                     if (C::I8) ptx::umma_i8_ts(d_tmem, at, bd, idesc, accum);
@@ -326,7 +347,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                                 }
                             }
                         }
-                        ptx::umma_commit(empty + s);
+                        ptx::umma_commit(used_b);
+                        if (!C::DENSE) ptx::umma_commit(used_a);
                     }
                     landed = __all_sync(0xffffffffu, next ? 1 : 0) != 0;
                 }
@@ -337,18 +359,18 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
     } else if (warp == 2) {
         // ---------------------------------------------------------------- TMA producer of the packed words
         if (!C::DENSE && lane == 0 && healthy) {
-            int rit = 0, e = 0;
+            int s = 0, e = 0;
+            uint32_t ph = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
                 const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
                 const int wrow = (int)(q.e * a.N) + q.n0;
-                for (int kb = 0; kb < nkb; kb += C::RAWK, rit++) {
-                    const int s = rit % (C::RAW_STAGES + C::DENSE);
-                    const uint32_t ph = (uint32_t)(rit / (C::RAW_STAGES + C::DENSE)) & 1u;
-                    ok = ptx::mbar_wait(raw_empty + s, ph ^ 1u, a.status);
+                for (int kb = 0; kb < nkb; kb += C::RAWK) {
+                    ok = ptx::mbar_wait_idle(raw_empty + s, ph, a.status);
                     if (!ok) break;
                     ptx::mbar_arrive_expect_tx(raw_full + s, (uint32_t)C::RAW_BYTES);
-                    ptx::tma_load_2d(smem + C::RAW_OFF + s * C::RAW_BYTES, &tmap_w, raw_full + s, kb * (C::RAW_ROW / 4), wrow);
+                    ptx::tma_load_2d(smem + C::RAW_OFF + s * C::RAW_BYTES, &maps.w, raw_full + s, kb * (C::RAW_ROW / 4), wrow);
+                    if (++s == C::RAW_STAGES) { s = 0; ph ^= 1u; }
                 }
             }
         }
@@ -369,7 +391,7 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                     if (j < C::KB) {
                     // even lanes wait for the packed words, odd lanes until the MMAs that read this stage last are done; a
                     // set whose k-block lies beyond the unit waits (and reports) as well, or it would run a round ahead
-                    ok = ptx::mbar_wait_warp((lane & 1) ? empty + s : raw_full + rs, (lane & 1) ? ph ^ 1u : rph, a.status);
+                    ok = ptx::mbar_wait_warp((lane & 1) ? taken + s : raw_full + rs, (lane & 1) ? ph ^ 1u : rph, a.status);
                     if (!ok) break;
                     seen = true;
                     if (kb0 + st + j < nkb) {
@@ -421,12 +443,12 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
                     if (lane == 0) ptx::mbar_arrive(ready + s);
                     }
                     it++;
-                    if (++s == C::STAGES) { s = 0; ph ^= 1u; }
+                    if (++s == C::NA) { s = 0; ph ^= 1u; }
                 }
                 if (ok && !seen) ok = ptx::mbar_wait_warp(raw_full + rs, rph, a.status);
                 __syncwarp();
                 if (ok && lane == 0) ptx::mbar_arrive(raw_empty + rs);
-                if (++rs == C::RAW_STAGES + C::DENSE) { rs = 0; rph ^= 1u; }
+                if (++rs == C::RAW_STAGES) { rs = 0; rph ^= 1u; }
             }
         }
     } else if (warp >= C::FIRST_EPI) {
@@ -448,7 +470,8 @@ scaled_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_cons
             }
             if (!C::I8) sc *= 0.5f;                      // bf16 weights are carried as +-2
             const int buf = C::ACC_BUFS == 2 ? (ti & 1) : 0;
-            ok = ptx::mbar_wait_warp(acc_full + buf, (uint32_t)(C::ACC_BUFS == 2 ? (ti >> 1) : ti) & 1u, a.status);
+            ok = ptx::mbar_wait_idle(acc_full + buf, (uint32_t)(C::ACC_BUFS == 2 ? (ti >> 1) : ti) & 1u, a.status);
+            ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN);
@@ -517,20 +540,21 @@ struct ScaledProblem {
 template <int WK, int BN>
 static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     using C = ScaledCfg<WK, BN>;
-    const ScaledArgs &a = p.a;
-    CUtensorMap mx, ms, mw;
+    ScaledArgs a = p.a;
+    ScaledMaps maps;
     const CUtensorMapDataType xt = C::I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const uint64_t xpitch = (uint64_t)p.ldx * (C::I8 ? 1 : 2);
-    const bool okx = make_map_2d(&mx, xt, p.X, (uint64_t)a.K, (uint64_t)a.M, xpitch, C::BK, BN, CU_TENSOR_MAP_SWIZZLE_128B) &&
-                     make_map_2d(&ms, xt, p.X, (uint64_t)a.K, (uint64_t)a.M, xpitch, C::BK, C::SMALL, CU_TENSOR_MAP_SWIZZLE_128B);
+    const int xe = C::I8 ? 1 : 2, box[3] = {C::BOX0, C::BOX1, C::BOX2};
+    a.wide = a.K % C::BK == 0;
+    for (int i = 0; i < 3; i++)
+        if (!make_map_blocks(maps.x + i, xt, xe, p.X, (uint64_t)a.K, (uint64_t)a.M, (uint64_t)p.ldx * xe, C::BK, box[i], C::KB, a.wide))
+            return TMQ_ERR_LAUNCH;
     const uint64_t wrows = (uint64_t)a.groups * (uint64_t)a.N;
     const bool okw = C::DENSE
-        ? make_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.W, (uint64_t)a.K, wrows, (uint64_t)p.ldw, C::BK, kTileC,
-                      CU_TENSOR_MAP_SWIZZLE_128B)
-        : make_map_2d(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.W, (uint64_t)prepack_valid_words(a.K), wrows,
+        ? make_map_blocks(&maps.w, xt, 1, p.W, (uint64_t)a.K, wrows, (uint64_t)p.ldw, C::BK, kTileC, C::KB, a.wide)
+        : make_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.W, (uint64_t)prepack_valid_words(a.K), wrows,
                       (uint64_t)prepack_row_words(a.K, C::I8 ? 1 : 0) * 4, C::DENSE ? 4 : C::RAW_PITCH / 4, kTileC,
                       C::RAW_PITCH == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
-    if (!okx || !okw) return TMQ_ERR_LAUNCH;
+    if (!okw) return TMQ_ERR_LAUNCH;
     int rc = ensure_dynamic_smem(scaled_gemm_kernel<WK, BN>, C::bytes(kMaxGroups));
     if (rc != TMQ_OK) return rc;
     // at most (rows / BN + groups) row tiles; CTAs beyond the real count find nothing to do
@@ -546,7 +570,7 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, scaled_gemm_kernel<WK, BN>, mx, ms, mw, a));
+    return cuda_status(cudaLaunchKernelEx(&cfg, scaled_gemm_kernel<WK, BN>, maps, a));
 }
 
 template <int WK>
@@ -554,7 +578,8 @@ static int dispatch_scaled(const ScaledProblem &p, cudaStream_t st) {
     const long long per_group = (p.a.M + p.a.groups - 1) / p.a.groups;
     if (per_group > 128) return launch_scaled<WK, 256>(p, st);
     if (per_group > 64) return launch_scaled<WK, 128>(p, st);
-    return launch_scaled<WK, 64>(p, st);
+    if (per_group > 32) return launch_scaled<WK, 64>(p, st);
+    return launch_scaled<WK, 32>(p, st);
 }
 
 static int check_scaled(const ScaledProblem &p, int x_bytes, bool dense) {
@@ -580,7 +605,7 @@ using namespace tmq;
 extern "C" int tmq_ternary_gemm_a8(const int8_t *X, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
                                    const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy,
                                    int *status, void *stream) {
-    const ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, status}};
+    const ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, status}};
     const int rc = check_scaled(p, 1, false);
     if (rc != TMQ_OK || M == 0) return rc;
     return dispatch_scaled<W_TERNARY_I8>(p, (cudaStream_t)stream);
@@ -589,7 +614,7 @@ extern "C" int tmq_ternary_gemm_a8(const int8_t *X, int64_t ldx, const float *ro
 extern "C" int tmq_gemm_i8(const int8_t *X, int64_t ldx, const float *row_scale, const int8_t *W, int64_t ldw,
                            const float *scale, const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K,
                            int64_t ldy, int *status, void *stream) {
-    const ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, status}};
+    const ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, status}};
     const int rc = check_scaled(p, 1, true);
     if (rc != TMQ_OK || M == 0) return rc;
     return dispatch_scaled<W_DENSE_I8>(p, (cudaStream_t)stream);
@@ -600,7 +625,7 @@ extern "C" int tmq_ternary_gemm_grouped_bf16(const void *X, int64_t ldx, const u
                                              int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest,
                                              int *status, void *stream) {
     const ScaledProblem p = {X, Wt, ldx, 0,
-                             {nullptr, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, status}};
+                             {nullptr, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 2, false);
     if (rc != TMQ_OK || M == 0) return rc;
@@ -613,7 +638,7 @@ extern "C" int tmq_ternary_gemm_grouped_a8(const int8_t *X, int64_t ldx, const f
                                            int groups, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy,
                                            int zero_rest, int *status, void *stream) {
     const ScaledProblem p = {X, Wt, ldx, 0,
-                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, status}};
+                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 1, false);
     if (rc != TMQ_OK || M == 0) return rc;
@@ -626,7 +651,7 @@ extern "C" int tmq_gemm_grouped_i8(const int8_t *X, int64_t ldx, const float *ro
                                    void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest,
                                    int *status, void *stream) {
     const ScaledProblem p = {X, W, ldx, ldw,
-                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, status}};
+                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 1, true);
     if (rc != TMQ_OK || M == 0) return rc;

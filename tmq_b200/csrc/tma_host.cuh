@@ -38,4 +38,19 @@ inline bool make_map_2d(CUtensorMap *map, CUtensorMapDataType dt, const void *ba
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Rows of `inner` elements as a 3-D tensor (element, row, k-block).  wide: the rows are cut into blocks of box_inner elements
+// (inner is a multiple of it) and one copy brings `blocks` of them, each as its own tile of box_rows rows; otherwise there is
+// one block, the copy's x coordinate walks along the row and elements beyond it are filled with zeros.
+inline bool make_map_blocks(CUtensorMap *map, CUtensorMapDataType dt, int elem, const void *base, uint64_t inner, uint64_t rows,
+                            uint64_t pitch_bytes, uint32_t box_inner, uint32_t box_rows, uint32_t blocks, bool wide) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    cuuint64_t dims[3] = {wide ? box_inner : inner, rows, wide ? inner / box_inner : 1};
+    cuuint64_t strides[2] = {pitch_bytes, (cuuint64_t)box_inner * elem};
+    cuuint32_t box[3] = {box_inner, box_rows, wide ? blocks : 1};
+    cuuint32_t estr[3] = {1, 1, 1};
+    return fn(map, dt, 3, const_cast<void *>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace tmq
