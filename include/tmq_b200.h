@@ -276,6 +276,16 @@ int tmq_gemm_i8(const int8_t *X, int64_t ldx, const float *row_scale, const int8
                 const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
                 void *stream);
 
+/* tmq_ternary_gemm_a8 for one to eight rows, quantisation included, in one launch: X of x_type TMQ_TYPE_* (quantised as
+ * tmq_quantize_rows does; any alignment; row_scale NULL) or x_type -1: int8 codes (16-byte aligned rows, ldx % 16 == 0) with
+ * row_scale.  Same results, bit for bit.  TMQ_ERR_UNSUPPORTED when an SM's share of the matrix exceeds its shared memory
+ * (N > 11840, or long rows): then quantise and call tmq_ternary_gemm_a8.  Wt is fetched ahead of the stream's previous kernel:
+ * the CONTRACT of tmq_ternary_gemv_bf16 holds (scale, bias, row_scale and X carry no such restriction).
+ * replaces: ternary_mvm_cuda, tmq/tmq_cuda.cu:563-603 (fp32 activations on CUDA cores). */
+int tmq_ternary_gemv_a8(const void *X, int x_type, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
+                        const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
+                        void *stream);
+
 /* Products grouped by expert: rows offsets[e] .. offsets[e + 1] - 1 of X use matrix e of the stacked weights
  * ([groups][N] rows, the layouts above; bf16: tmq_prepack fmt 0, X bf16 with ldx % 8 == 0), scale and bias [groups][N].
  * offsets: DEVICE array of groups + 1 boundaries, int32 or int64 (offsets_bytes = 4 or 8), read by the kernel only; groups

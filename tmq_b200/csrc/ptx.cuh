@@ -102,6 +102,21 @@ __device__ __forceinline__ bool mbar_wait_idle(uint64_t *bar, uint32_t parity, i
     }
 }
 
+// A wait for copies or MMAs this CTA itself has in flight: it does not end early because some other CTA failed (the CTA's
+// memory must not be handed on under them), only when the budget runs out.
+__device__ __forceinline__ bool mbar_wait_own(uint64_t *bar, uint32_t parity, int *status,
+                                              long long budget = kWaitBudgetCycles) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_wait(bar, parity)) {
+        if (clock64() - t0 > budget) {
+            atomicCAS(status, 0, TMQ_ERR_TIMEOUT);
+            return false;
+        }
+    }
+    return true;
+}
+
 // mbar_wait made by a whole converged warp, with a warp-uniform result (one lane giving up makes every lane give up),
 // so that code after it can stay convergent (elect_one needs the full warp).
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, int *status,

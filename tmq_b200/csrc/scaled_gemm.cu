@@ -225,7 +225,8 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
     uint64_t *raw_empty = raw_full + C::RAW_STAGES;
     uint64_t *acc_full = raw_empty + C::RAW_STAGES;                           // [2]
     uint64_t *acc_empty = acc_full + 2;                                       // [2]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
+    uint64_t *drain = acc_empty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
     int *begin = reinterpret_cast<int *>(smem + C::TAB_OFF);
     int *tiles = begin + a.groups + 1;
 
@@ -251,6 +252,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             ptx::mbar_init(acc_full + b, 1);
             ptx::mbar_init(acc_empty + b, C::EPI);
         }
+        ptx::mbar_init(drain, 1);
         ptx::fence_mbar_init();
         for (int i = 0; i < 3; i++) ptx::prefetch_tensormap(maps.x + i);
         ptx::prefetch_tensormap(&maps.w);
@@ -271,7 +273,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
         if (lane == 0 && healthy) {
-            int s = 0, e = 0;
+            int s = 0, e = 0, round = 0;
             uint32_t ph = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
@@ -295,9 +297,13 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                             ptx::tma_load_3d(xd + j * rows * kOpRow, mx, full + s, (kb + j) * C::BK, q.row0, 0);
                         }
                     }
-                    if (++s == C::NB) { s = 0; ph ^= 1u; }
+                    if (++s == C::NB) { s = 0; ph ^= 1u; round = 1; }
                 }
             }
+            // gave up: wait for the copies still on their way (ph: parity of this round's slots waiting to be refilled)
+            if (!ok)
+                for (int i = 0; i < C::NB; i++)
+                    if (round || i < s) ptx::mbar_wait_own(full + i, i < s ? ph ^ 1u : ph, a.status);
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (whole warp walks, one lane issues)
@@ -355,11 +361,17 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                 if (ok && ptx::elect_one()) ptx::umma_commit(acc_full + buf);
                 __syncwarp();
             }
+            if (!ok) {                                   // gave up: the MMAs issued so far end before anything is freed
+                if (ptx::elect_one()) ptx::umma_commit(drain);
+                __syncwarp();
+                ptx::mbar_wait_own(drain, 0, a.status);
+                __syncwarp();
+            }
         }
     } else if (warp == 2) {
         // ---------------------------------------------------------------- TMA producer of the packed words
         if (!C::DENSE && lane == 0 && healthy) {
-            int s = 0, e = 0;
+            int s = 0, e = 0, round = 0;
             uint32_t ph = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
@@ -370,9 +382,12 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                     if (!ok) break;
                     ptx::mbar_arrive_expect_tx(raw_full + s, (uint32_t)C::RAW_BYTES);
                     ptx::tma_load_2d(smem + C::RAW_OFF + s * C::RAW_BYTES, &maps.w, raw_full + s, kb * (C::RAW_ROW / 4), wrow);
-                    if (++s == C::RAW_STAGES) { s = 0; ph ^= 1u; }
+                    if (++s == C::RAW_STAGES) { s = 0; ph ^= 1u; round = 1; }
                 }
             }
+            if (!ok)
+                for (int i = 0; i < C::RAW_STAGES; i++)
+                    if (round || i < s) ptx::mbar_wait_own(raw_full + i, i < s ? ph ^ 1u : ph, a.status);
         }
     } else if (!C::DENSE && warp >= 4 && warp < C::FIRST_EPI) {
         // ---------------------------------------------------------------- decode

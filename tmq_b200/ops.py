@@ -488,8 +488,9 @@ class _StatusWatch:
 
 def _launched(device):
     """Book-keeping after a tensor-core launch on `device` (see _StatusWatch)."""
-    device = torch.device(device)
-    key = device.index if device.index is not None else torch.cuda.current_device()
+    key = device.index if isinstance(device, torch.device) else torch.device(device).index
+    if key is None:
+        key = torch.cuda.current_device()
     w = _watch.get(key)
     if w is None:
         w = _watch[key] = _StatusWatch(torch.device("cuda", key))
@@ -742,53 +743,68 @@ def ternary_gemv_batched(x, wts, columns, scales=None, biases=None, out_dtype=to
 # ------------------------------------------------------------------------------------------------ 8-bit products
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # TMQ_TYPE_*
+_A8_TYPES = {torch.int8: -1, **_TYPES}
 I8_K_MAX = 131071        # int32 sums of 8-bit products are exact up to this length
 GROUPS_MAX = 512         # experts one grouped launch takes (TMQ_GROUPS_MAX)
+A8_TOKENS = 8            # rows the one-launch form (tmq_ternary_gemv_a8) takes
+_row_words = {}
+_status_address = {}
+
+# The calls below are a few microseconds long for single tokens: their host side avoids everything that costs as much
+# (torch.empty with a shape tuple, stream objects, device contexts for the device that is current anyway).
 
 
-def _enqueue(fn, device, what, *args):
-    """fn(*args, stream) on the current stream of `device`, which is made the current device for the call."""
-    index = device.index
+def _enqueue(fn, index, *args):
+    """fn(*args, status word, stream) on the current stream of device `index`, which is made the current device for the call;
+    returns the status."""
+    word = _status_address.get(index)
+    if word is None:
+        word = _status_address[index] = gemm_status_word(torch.device("cuda", index)).data_ptr()
     if torch.cuda.current_device() == index:
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if rc:
-        check(rc, what)
+        return fn(*args, word, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, word, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _vector(name, what, t, shape, device):
-    """Device pointer holder of an optional fp32 vector: (tensor or None, address or None)."""
+    """(tensor, address) of an optional fp32 vector; the tensor is to be kept until the launch."""
     if t is None:
         return None, None
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise RuntimeError(f"{name}: {what} must have shape {list(shape)}")
-    if t.dtype != torch.float32 or t.device != device or not t.is_contiguous():
+    if t.dtype is not torch.float32 or t.device != device or not t.is_contiguous():
         t = t.detach().to(device=device, dtype=torch.float32).contiguous()
     return t, t.data_ptr()
 
 
-def _rows_in(name, x, dtypes):
-    if not isinstance(x, torch.Tensor) or x.device.type != "cuda" or x.dim() != 2 or x.dtype not in dtypes:
+def _rows_type(name, x, types):
+    """TMQ_TYPE of a 2-D CUDA tensor (-1: int8) or a refusal."""
+    code = types.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if code is None or not x.is_cuda or x.dim() != 2:
         raise RuntimeError(f"{name}: expected a 2-D CUDA activation tensor of type "
-                           + " / ".join(str(d).replace("torch.", "") for d in dtypes))
+                           + " / ".join(str(d).replace("torch.", "") for d in types))
     if x.shape[1] == 0:
         raise RuntimeError(f"{name}: rows without elements")
+    return code
 
 
-def _aligned_rows(x):
+def _unit_rows(x, M, K):
+    """(tensor, row stride) with unit column stride and rows that do not overlap."""
+    if (x.stride(1) != 1 and K > 1) or (M > 1 and x.stride(0) < K):
+        x = x.contiguous()
+    return x, x.stride(0) if M > 1 else (K + 15) // 16 * 16
+
+
+def _aligned_rows(x, M, K):
     """(tensor, row stride) of rows the TMA path can read: unit column stride, 16-byte aligned rows that do not overlap.
     Anything else is copied into such rows first."""
-    M, K = x.shape
-    esz = x.element_size()
-    lanes = 16 // esz
-    if x.stride(1) == 1 or K == 1:
-        if x.data_ptr() % 16 == 0:
-            if M == 1:
-                return x, (K + lanes - 1) // lanes * lanes
-            if x.stride(0) >= K and x.stride(0) % lanes == 0:
-                return x, x.stride(0)
+    lanes = 16 // x.element_size()
+    if (x.stride(1) == 1 or K == 1) and x.data_ptr() % 16 == 0:
+        if M == 1:
+            return x, (K + lanes - 1) // lanes * lanes
+        ld = x.stride(0)
+        if ld >= K and ld % lanes == 0:
+            return x, ld
     kp = (K + lanes - 1) // lanes * lanes
     rows = torch.empty((M, kp), dtype=x.dtype, device=x.device)
     rows[:, :K].copy_(x)
@@ -796,15 +812,24 @@ def _aligned_rows(x):
 
 
 def _rows_out(name, out, M, N, dtype, device):
-    """(tensor, row stride) of the result: fresh, or the caller's `out` with rows of any stride."""
-    if dtype not in _TYPES:
+    """(tensor, row stride, TMQ_TYPE) of the result: fresh, or the caller's `out` with rows of any stride."""
+    code = _TYPES.get(dtype)
+    if code is None:
         raise ValueError(f"{name}: output dtype must be float32, bfloat16 or float16")
     if out is None:
-        return torch.empty((M, N), dtype=dtype, device=device), N
+        return torch.empty_strided((M, N), (N, 1), dtype=dtype, device=device), N, code
     if out.dtype != dtype or out.device != device or out.dim() != 2 or tuple(out.shape) != (M, N) or \
             (N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
         raise RuntimeError(f"{name}: `out` must be an [M, N] tensor of the output dtype with unit column stride")
-    return out, out.stride(0) if M > 1 else N
+    return out, out.stride(0) if M > 1 else N, code
+
+
+def _check_packed(name, wt, N, K, fmt, device):
+    words = _row_words.get((K, fmt))
+    if words is None:
+        words = _row_words[(K, fmt)] = prepack_row_words(K, fmt)
+    if wt.dtype is not torch.int32 or wt.shape[-2:] != (N, words) or not wt.is_contiguous() or wt.device != device:
+        raise RuntimeError(f"{name}: prepacked weights do not match the problem's shape, kind or device")
 
 
 def quantize_rows(x, out=None):
@@ -813,68 +838,76 @@ def quantize_rows(x, out=None):
     that holds a NaN or an infinity gets scale NaN (and codes 0), so products of that row are NaN.  The codes are a view of
     rows padded to a multiple of 16 bytes, the form the 8-bit products read in place.  The rows of a weight matrix are its
     output channels: quantize_rows(weight) makes the operands of gemm_i8.  out: optional (codes, scale) to write into, codes
-    with unit column stride; padding columns of `out` are not touched."""
-    _rows_in("quantize_rows", x, (torch.float32, torch.bfloat16, torch.float16))
-    if x.stride(1) != 1 and x.shape[1] > 1:
-        x = x.contiguous()
+    with unit column stride; padding columns of `out` are not touched.  No gradient."""
+    code = _rows_type("quantize_rows", x, _TYPES)
     M, K = x.shape
+    dev = x.device
     if out is None:
-        kp = (K + 15) // 16 * 16
-        rows = torch.empty((M, kp), dtype=torch.int8, device=x.device)
-        scale = torch.empty(M, dtype=torch.float32, device=x.device)
-        q, width = (rows if kp == K else rows[:, :K]), kp
+        kp = width = ldq = (K + 15) // 16 * 16
+        q = torch.empty_strided((M, K), (kp, 1), dtype=torch.int8, device=dev) if kp == K else \
+            torch.empty_strided((M, kp), (kp, 1), dtype=torch.int8, device=dev)[:, :K]
+        scale = torch.empty_strided((M,), (1,), dtype=torch.float32, device=dev)
     else:
         q, scale = out
-        if q.dtype != torch.int8 or q.device != x.device or tuple(q.shape) != (M, K) or (K > 1 and q.stride(1) != 1) or \
-                (M > 1 and q.stride(0) < K) or scale.dtype != torch.float32 or scale.device != x.device or \
+        if q.dtype != torch.int8 or q.device != dev or tuple(q.shape) != (M, K) or (K > 1 and q.stride(1) != 1) or \
+                (M > 1 and q.stride(0) < K) or scale.dtype != torch.float32 or scale.device != dev or \
                 tuple(scale.shape) != (M,) or not scale.is_contiguous():
             raise RuntimeError("quantize_rows: `out` must be (int8 [M, K] with unit column stride, float32 [M])")
         width = K
+        ldq = q.stride(0) if M > 1 else (K + 15) // 16 * 16
     if M:
-        ldx = x.stride(0) if M > 1 else (K + 15) // 16 * 16
-        ldq = q.stride(0) if M > 1 else (width + 15) // 16 * 16
-        if ldx < K:                                   # expanded rows
-            x = x.contiguous()
-            ldx = K
-        _enqueue(lib().tmq_quantize_rows, x.device, "quantize_rows", x.data_ptr(), _TYPES[x.dtype], q.data_ptr(),
-                 scale.data_ptr(), M, K, ldx, ldq, width)
+        x, ldx = _unit_rows(x, M, K)
+        index = dev.index
+        args = (x.data_ptr(), code, q.data_ptr(), scale.data_ptr(), M, K, ldx, ldq, width)
+        if torch.cuda.current_device() == index:
+            rc = lib().tmq_quantize_rows(*args, torch._C._cuda_getCurrentRawStream(index))
+        else:
+            with torch.cuda.device(index):
+                rc = lib().tmq_quantize_rows(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc:
+            check(rc, "quantize_rows")
     return q, scale
-
-
-def _a8_operands(name, x, row_scale):
-    """int8 rows and their scales: as given, or quantised here from floating point."""
-    _rows_in(name, x, (torch.int8, torch.float32, torch.bfloat16, torch.float16))
-    if x.dtype != torch.int8:
-        if row_scale is not None:
-            raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
-        x, row_scale = quantize_rows(x)
-    if x.shape[1] > I8_K_MAX:
-        raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
-    return x, row_scale
 
 
 def ternary_gemm_a8(x, wt, columns, row_scale=None, scale=None, bias=None, out_dtype=torch.bfloat16, out=None):
     """Y[m][n] = row_scale[m] * scale[n] * sum_k x[m][k] T[n][k] + bias[n] with 8-bit activations and packed ternary
     weights; the sums are exact, the scaling is fp32, the result bf16, fp16 or fp32 [M, columns].
     x: CUDA int8 [M, K] (any row stride; row_scale fp32 [M] or None for 1), or fp32 / bf16 / fp16 [M, K], which is quantised
-    here exactly as quantize_rows does.  wt: prepack(..., FMT_I8).  scale, bias: fp32 [columns] or None.  out: optional
-    [M, columns] tensor of the output dtype whose rows may be strided.  No gradient."""
-    x, row_scale = _a8_operands("ternary_gemm_a8", x, row_scale)
+    here exactly as quantize_rows does (inside the product's launch for up to A8_TOKENS rows).  wt: prepack(..., FMT_I8).
+    scale, bias: fp32 [columns] or None.  out: optional [M, columns] tensor of the output dtype whose rows may be strided.
+    No gradient."""
+    name = "ternary_gemm_a8"
+    code = _rows_type(name, x, _A8_TYPES)
+    if code >= 0 and row_scale is not None:
+        raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
     M, K = x.shape
+    if K > I8_K_MAX:
+        raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
     N = int(columns)
-    _check_weights("ternary_gemm_a8", wt, N, K, FMT_I8)
-    if wt.device != x.device:
-        raise RuntimeError("ternary_gemm_a8: weights on another device than the activations")
     dev = x.device
-    rs, p_rs = _vector("ternary_gemm_a8", "row_scale", row_scale, (M,), dev)
-    sc, p_sc = _vector("ternary_gemm_a8", "scale", scale, (N,), dev)
-    bi, p_bi = _vector("ternary_gemm_a8", "bias", bias, (N,), dev)
-    y, ldy = _rows_out("ternary_gemm_a8", out, M, N, out_dtype, dev)
+    _check_packed(name, wt, N, K, FMT_I8, dev)
+    if wt.dim() != 2:
+        raise RuntimeError(f"{name}: expected the prepacked weights of one matrix")
+    rs, p_rs = _vector(name, "row_scale", row_scale, (M,), dev)
+    sc, p_sc = _vector(name, "scale", scale, (N,), dev)
+    bi, p_bi = _vector(name, "bias", bias, (N,), dev)
+    y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
-    x, ldx = _aligned_rows(x)
-    _enqueue(lib().tmq_ternary_gemm_a8, dev, "ternary_gemm_a8", x.data_ptr(), ldx, p_rs, wt.data_ptr(), p_sc, p_bi,
-             y.data_ptr(), _TYPES[y.dtype], M, N, K, ldy, gemm_status_word(dev).data_ptr())
+    rc = -6
+    if M <= A8_TOKENS:
+        x, ldx = _aligned_rows(x, M, K) if code < 0 else _unit_rows(x, M, K)
+        rc = _enqueue(lib().tmq_ternary_gemv_a8, dev.index, x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi,
+                      y.data_ptr(), y_code, M, N, K, ldy)
+    if rc == -6:               # more rows, or a matrix whose share per SM exceeds its shared memory
+        if code >= 0:
+            x, rs = quantize_rows(x)
+            p_rs = rs.data_ptr()
+        x, ldx = _aligned_rows(x, M, K)
+        rc = _enqueue(lib().tmq_ternary_gemm_a8, dev.index, x.data_ptr(), ldx, p_rs, wt.data_ptr(), p_sc, p_bi, y.data_ptr(),
+                      y_code, M, N, K, ldy)
+    if rc:
+        check(rc, name)
     _launched(dev)
     return y
 
@@ -898,22 +931,32 @@ def _check_i8_weights(name, w, dims, device):
 def gemm_i8(x, weight, row_scale=None, scale=None, bias=None, out_dtype=torch.bfloat16, out=None):
     """ternary_gemm_a8 for 8-bit weights: weight int8 [N, K] with rows that start at multiples of 16 bytes (what
     quantize_rows returns), scale fp32 [N] per channel.  Everything else as there."""
-    x, row_scale = _a8_operands("gemm_i8", x, row_scale)
+    name = "gemm_i8"
+    code = _rows_type(name, x, _A8_TYPES)
+    if code >= 0 and row_scale is not None:
+        raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
     M, K = x.shape
+    if K > I8_K_MAX:
+        raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
     dev = x.device
-    ldw = _check_i8_weights("gemm_i8", weight, 2, dev)
+    ldw = _check_i8_weights(name, weight, 2, dev)
     N = weight.shape[0]
     if weight.shape[1] != K:
-        raise RuntimeError("gemm_i8: activation width does not match the weights")
-    rs, p_rs = _vector("gemm_i8", "row_scale", row_scale, (M,), dev)
-    sc, p_sc = _vector("gemm_i8", "scale", scale, (N,), dev)
-    bi, p_bi = _vector("gemm_i8", "bias", bias, (N,), dev)
-    y, ldy = _rows_out("gemm_i8", out, M, N, out_dtype, dev)
+        raise RuntimeError(f"{name}: activation width does not match the weights")
+    rs, p_rs = _vector(name, "row_scale", row_scale, (M,), dev)
+    sc, p_sc = _vector(name, "scale", scale, (N,), dev)
+    bi, p_bi = _vector(name, "bias", bias, (N,), dev)
+    y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
-    x, ldx = _aligned_rows(x)
-    _enqueue(lib().tmq_gemm_i8, dev, "gemm_i8", x.data_ptr(), ldx, p_rs, weight.data_ptr(), ldw, p_sc, p_bi, y.data_ptr(),
-             _TYPES[y.dtype], M, N, K, ldy, gemm_status_word(dev).data_ptr())
+    if code >= 0:
+        x, rs = quantize_rows(x)
+        p_rs = rs.data_ptr()
+    x, ldx = _aligned_rows(x, M, K)
+    rc = _enqueue(lib().tmq_gemm_i8, dev.index, x.data_ptr(), ldx, p_rs, weight.data_ptr(), ldw, p_sc, p_bi, y.data_ptr(),
+                  y_code, M, N, K, ldy)
+    if rc:
+        check(rc, name)
     _launched(dev)
     return y
 
@@ -937,32 +980,35 @@ def ternary_gemm_grouped(x, wts, columns, offsets, row_scale=None, scales=None, 
     replay.  Groups may be empty.  scales, biases: fp32 [experts, columns] or None.  Rows outside every group are zero in a
     fresh result and left as they were in `out`.  Boundaries outside 0 .. M or out of order give empty or shortened groups.
     No gradient."""
-    _rows_in("ternary_gemm_grouped", x, (torch.bfloat16, torch.int8))
-    i8 = x.dtype == torch.int8
+    name = "ternary_gemm_grouped"
+    i8 = _rows_type(name, x, {torch.bfloat16: 1, torch.int8: -1}) < 0
     M, K = x.shape
     N = int(columns)
     dev = x.device
-    if not isinstance(wts, torch.Tensor) or wts.dim() != 3 or wts.device != dev or not wts.is_contiguous():
-        raise RuntimeError("ternary_gemm_grouped: expected the stacked prepacked weights [experts, columns, row words] on the "
-                           "activations' device")
+    if not isinstance(wts, torch.Tensor) or wts.dim() != 3:
+        raise RuntimeError(f"{name}: expected the stacked prepacked weights [experts, columns, row words]")
     E = wts.shape[0]
-    _check_offsets("ternary_gemm_grouped", offsets, E, dev)
-    _check_weights("ternary_gemm_grouped", wts[0], N, K, FMT_I8 if i8 else FMT_BF16)
+    _check_offsets(name, offsets, E, dev)
+    _check_packed(name, wts, N, K, FMT_I8 if i8 else FMT_BF16, dev)
     if i8 and K > I8_K_MAX:
-        raise RuntimeError(f"ternary_gemm_grouped: at most {I8_K_MAX} columns (int32 sums)")
+        raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
     if not i8 and row_scale is not None:
-        raise RuntimeError("ternary_gemm_grouped: row_scale belongs to int8 activations")
-    rs, p_rs = _vector("ternary_gemm_grouped", "row_scale", row_scale, (M,), dev)
-    sc, p_sc = _vector("ternary_gemm_grouped", "scales", scales, (E, N), dev)
-    bi, p_bi = _vector("ternary_gemm_grouped", "biases", biases, (E, N), dev)
-    y, ldy = _rows_out("ternary_gemm_grouped", out, M, N, out_dtype, dev)
+        raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
+    rs, p_rs = _vector(name, "row_scale", row_scale, (M,), dev)
+    sc, p_sc = _vector(name, "scales", scales, (E, N), dev)
+    bi, p_bi = _vector(name, "biases", biases, (E, N), dev)
+    y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
-    x, ldx = _aligned_rows(x)
-    head = (x.data_ptr(), ldx) + ((p_rs,) if i8 else ()) + (wts.data_ptr(), p_sc, p_bi)
-    _enqueue(lib().tmq_ternary_gemm_grouped_a8 if i8 else lib().tmq_ternary_gemm_grouped_bf16, dev, "ternary_gemm_grouped",
-             *head, offsets.data_ptr(), offsets.element_size(), E, y.data_ptr(), _TYPES[y.dtype], M, N, K, ldy,
-             1 if out is None else 0, gemm_status_word(dev).data_ptr())
+    x, ldx = _aligned_rows(x, M, K)
+    tail = (wts.data_ptr(), p_sc, p_bi, offsets.data_ptr(), offsets.element_size(), E, y.data_ptr(), y_code, M, N, K, ldy,
+            1 if out is None else 0)
+    if i8:
+        rc = _enqueue(lib().tmq_ternary_gemm_grouped_a8, dev.index, x.data_ptr(), ldx, p_rs, *tail)
+    else:
+        rc = _enqueue(lib().tmq_ternary_gemm_grouped_bf16, dev.index, x.data_ptr(), ldx, *tail)
+    if rc:
+        check(rc, name)
     _launched(dev)
     return y
 
@@ -970,24 +1016,26 @@ def ternary_gemm_grouped(x, wts, columns, offsets, row_scale=None, scales=None, 
 def gemm_i8_grouped(x, weights, offsets, row_scale=None, scales=None, biases=None, out_dtype=torch.bfloat16, out=None):
     """ternary_gemm_grouped for 8-bit weights: weights int8 [experts, N, K] whose rows lie one behind the other and start at
     multiples of 16 bytes; x int8 [M, K] with row_scale fp32 [M].  Everything else as there."""
-    _rows_in("gemm_i8_grouped", x, (torch.int8,))
+    name = "gemm_i8_grouped"
+    _rows_type(name, x, {torch.int8: -1})
     M, K = x.shape
     dev = x.device
-    ldw = _check_i8_weights("gemm_i8_grouped", weights, 3, dev)
+    ldw = _check_i8_weights(name, weights, 3, dev)
     E, N = weights.shape[:2]
-    _check_offsets("gemm_i8_grouped", offsets, E, dev)
+    _check_offsets(name, offsets, E, dev)
     if weights.shape[2] != K or K > I8_K_MAX:
-        raise RuntimeError("gemm_i8_grouped: activation width does not match the weights or exceeds the int32 sums")
-    rs, p_rs = _vector("gemm_i8_grouped", "row_scale", row_scale, (M,), dev)
-    sc, p_sc = _vector("gemm_i8_grouped", "scales", scales, (E, N), dev)
-    bi, p_bi = _vector("gemm_i8_grouped", "biases", biases, (E, N), dev)
-    y, ldy = _rows_out("gemm_i8_grouped", out, M, N, out_dtype, dev)
+        raise RuntimeError(f"{name}: activation width does not match the weights or exceeds the int32 sums")
+    rs, p_rs = _vector(name, "row_scale", row_scale, (M,), dev)
+    sc, p_sc = _vector(name, "scales", scales, (E, N), dev)
+    bi, p_bi = _vector(name, "biases", biases, (E, N), dev)
+    y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
-    x, ldx = _aligned_rows(x)
-    _enqueue(lib().tmq_gemm_grouped_i8, dev, "gemm_i8_grouped", x.data_ptr(), ldx, p_rs, weights.data_ptr(), ldw, p_sc, p_bi,
-             offsets.data_ptr(), offsets.element_size(), E, y.data_ptr(), _TYPES[y.dtype], M, N, K, ldy,
-             1 if out is None else 0, gemm_status_word(dev).data_ptr())
+    x, ldx = _aligned_rows(x, M, K)
+    rc = _enqueue(lib().tmq_gemm_grouped_i8, dev.index, x.data_ptr(), ldx, p_rs, weights.data_ptr(), ldw, p_sc, p_bi,
+                  offsets.data_ptr(), offsets.element_size(), E, y.data_ptr(), y_code, M, N, K, ldy, 1 if out is None else 0)
+    if rc:
+        check(rc, name)
     _launched(dev)
     return y
 
