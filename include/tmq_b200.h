@@ -265,7 +265,7 @@ int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *scale, int64_
 /* Y[m][n] = acc * row_scale[m] * scale[n] + bias[n],  acc = sum_k X[m][k] W[n][k] exact in int32 (K <= 131071), then fp32:
  * (acc * row_scale) rounded, times scale plus bias in one fused multiply-add, rounded once more to y_type (TMQ_TYPE_*).
  * row_scale [M], scale [N], bias [N]: fp32, NULL for 1 / 1 / 0.  X int8 [M][ldx], 16-byte aligned, ldx % 16 == 0, any
- * K <= ldx (columns beyond K are not read).  Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw],
+ * K <= ldx (columns beyond K are not used).  Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw],
  * 16-byte aligned, ldw % 16 == 0.  Y [M][ldy], element-aligned.
  * *status: see "Status word" above.
  * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549, and the post_scale / bias of Linear.compact_forward, tmq/tmq.py:662-688. */

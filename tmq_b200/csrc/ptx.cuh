@@ -124,6 +124,47 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, i
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, budget) ? 1 : 0) != 0;
 }
 
+// The whole-warp wait and the arrival on shared-window addresses, for loops whose barrier addresses are stepped rather than
+// indexed: a decode warp's round is short enough that pointer arithmetic shows.
+__device__ __forceinline__ bool mbar_wait_warp_at(uint32_t bar, uint32_t parity, int *status,
+                                                  long long budget = kWaitBudgetCycles) {
+    long long t0 = 0;
+    bool ok = true;
+    for (uint32_t spin = 0;; spin++) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.b32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) break;
+        if (spin == 0) t0 = clock64();
+        if ((spin & 0x3FFu) == 0x3FFu) {
+            ok = *reinterpret_cast<volatile int *>(status) == 0;
+            if (ok && clock64() - t0 > budget) {
+                atomicCAS(status, 0, TMQ_ERR_TIMEOUT);
+                ok = false;
+            }
+            if (!ok) break;
+        }
+    }
+    return __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint4 lds_v4(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+
+__device__ __forceinline__ void sts_v4(uint32_t addr, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+
 // ---------------------------------------------------------------------------------------------------- fences / TMA
 
 __device__ __forceinline__ void fence_proxy_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

@@ -1,0 +1,110 @@
+// What the kernels of the scaled and grouped products share: their arguments, the table of work units that the group
+// boundaries make, element stores.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace tmq {
+
+enum { W_TERNARY_BF16 = 0, W_TERNARY_I8 = 1, W_DENSE_I8 = 2 };
+
+constexpr int kMaxGroups = TMQ_GROUPS_MAX;
+
+struct ScaledArgs {
+    const float *row_scale;          // [M] or null (1)
+    const float *scale, *bias;       // [groups][N] or null (1 / 0)
+    void *Y;
+    const void *offsets;             // [groups + 1] int32 or int64, null: one group of all rows
+    long long M, N, K, ldy;
+    int groups, offsets64, y_type, zero_rest;
+    int wide;                        // K is whole k-blocks: one box per stage
+    int *status;
+};
+
+// A product as the C entry points describe it.
+struct ScaledProblem {
+    const void *X, *W;
+    long long ldx, ldw;              // row strides of X (elements) and of 8-bit weights (bytes)
+    ScaledArgs a;
+};
+
+int launch_scaled_skinny(int kind, const ScaledProblem &p, cudaStream_t st);
+
+#ifdef __CUDACC__
+// Unit u of the launch: rows [row0, row0 + rows) of group e, channels [n0, n0 + tile_c).
+struct Unit {
+    int e, row0, rows, n0;
+};
+// begin[e]: first row of group e, begin[groups]: end of the last; tiles[e]: row tiles before group e.  `e` only moves forward.
+__device__ __forceinline__ Unit locate(int u, int &e, const int *begin, const int *tiles, int tiles_n, int bn, int tile_c) {
+    const int rt = u / tiles_n;
+    while (tiles[e + 1] <= rt) e++;
+    Unit q;
+    q.e = e;
+    q.n0 = (u - rt * tiles_n) * tile_c;
+    q.row0 = begin[e] + (rt - tiles[e]) * bn;
+    const int left = begin[e + 1] - q.row0;
+    q.rows = left < bn ? left : bn;
+    return q;
+}
+
+// Executed by one warp: boundaries -> table.  Chunks of 32 boundaries, a running maximum and a running sum of tiles.
+__device__ __forceinline__ void build_table(const ScaledArgs &a, int *begin, int *tiles, int bn, int lane) {
+    if (!a.offsets) {
+        if (lane == 0) {
+            begin[0] = 0; begin[1] = (int)a.M;
+            tiles[0] = 0; tiles[1] = (int)((a.M + bn - 1) / bn);
+        }
+        return;
+    }
+    int run = 0, sum = 0;                                       // running maximum of the boundaries, tiles so far
+    for (int c = 0; c <= a.groups; c += 32) {
+        const int i = c + lane;
+        long long v = 0;
+        if (i <= a.groups)
+            v = a.offsets64 ? reinterpret_cast<const long long *>(a.offsets)[i] : reinterpret_cast<const int *>(a.offsets)[i];
+        int b = (int)(v < 0 ? 0 : v > a.M ? a.M : v);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, b, o);
+            if (lane >= o) b = max(b, x);
+        }
+        b = max(b, run);
+        int prev = __shfl_up_sync(0xffffffffu, b, 1);
+        if (lane == 0) prev = run;
+        int t = (i == 0 || i > a.groups) ? 0 : (b - prev + bn - 1) / bn;      // tiles of group i - 1
+        const int last = __shfl_sync(0xffffffffu, b, 31);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, t, o);
+            if (lane >= o) t += x;
+        }
+        if (i <= a.groups) {
+            begin[i] = b;
+            tiles[i] = sum + t;
+        }
+        sum += __shfl_sync(0xffffffffu, t, 31);
+        run = last;
+    }
+}
+
+__device__ __forceinline__ void store_one(void *Y, int y_type, long long i, float f) {
+    if (y_type == TMQ_TYPE_F32) reinterpret_cast<float *>(Y)[i] = f;
+    else if (y_type == TMQ_TYPE_BF16) reinterpret_cast<__nv_bfloat16 *>(Y)[i] = __float2bfloat16_rn(f);
+    else reinterpret_cast<__half *>(Y)[i] = __float2half_rn(f);
+}
+
+
+// Rows before the first and behind the last group of a fresh result, dealt over the CTAs and `threads` threads of each.
+__device__ __forceinline__ void zero_rest_rows(const ScaledArgs &a, const int *begin, int thread, int threads) {
+    const long long lead = begin[0], tail = begin[a.groups], total = lead + (a.M - tail);
+    for (long long r = blockIdx.x; r < total; r += gridDim.x) {
+        const long long m = r < lead ? r : tail + (r - lead);
+        for (long long n = thread; n < a.N; n += threads) store_one(a.Y, a.y_type, m * a.ldy + n, 0.0f);
+    }
+}
+#endif
+
+}  // namespace tmq

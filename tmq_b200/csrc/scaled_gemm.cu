@@ -23,32 +23,23 @@
 #include "common.cuh"
 #include "decode.cuh"
 #include "ptx.cuh"
+#include "scaled_common.cuh"
 #include "tma_host.cuh"
 
 namespace tmq {
 
-enum { W_TERNARY_BF16 = 0, W_TERNARY_I8 = 1, W_DENSE_I8 = 2 };
-
 constexpr int kTileC = 128;          // channels of a unit (MMA M)
 constexpr int kOpRow = 128;          // bytes of one operand row per k-block: 64 bf16 or 128 int8
 constexpr int kRowStep = 32;         // granularity of a unit's MMA N
-constexpr int kMaxGroups = TMQ_GROUPS_MAX;
 
 // Tensor maps of a launch.  A TMA instruction costs about 200 cycles of its unit whatever it brings (bf16 tiles of 32 rows
 // with one box per k-block: 154 ns per k-block), so a box spans all k-blocks of a stage where the row length allows it.
+// Activation boxes come in three heights (multiples of 8: the swizzle's period), a unit takes the lowest that holds its
+// rows.  Rows of a box that lie outside the matrix cost about ten cycles each (one row of 11008 x 4096 8-bit weights: 12.8 us
+// with a box of 32), so a plain product's last tile gets a box of its own height.
 struct ScaledMaps {
     CUtensorMap x[3], w;
-};
-
-struct ScaledArgs {
-    const float *row_scale;          // [M] or null (1)
-    const float *scale, *bias;       // [groups][N] or null (1 / 0)
-    void *Y;
-    const void *offsets;             // [groups + 1] int32 or int64, null: one group of all rows
-    long long M, N, K, ldy;
-    int groups, offsets64, y_type, zero_rest;
-    int wide;                        // K is whole k-blocks: one box per stage
-    int *status;
+    int height[3];
 };
 
 template <int WK, int BN>
@@ -75,22 +66,21 @@ struct ScaledCfg {
     static constexpr int A_BYTES = TA ? 0 : kTileC * kOpRow;                     // of one k-block
     static constexpr int B_BYTES = BN * kOpRow;
     static constexpr int RAW_BYTES = kTileC * RAW_PITCH;
-    // heights of the activation boxes: a unit takes the lowest that holds its rows
-    static constexpr int BOX0 = BN, BOX1 = BN > 32 ? BN / 2 : 32, BOX2 = BN > 64 ? BN / 4 : 32;
     static constexpr int ACC_BUFS = (TA && BN > 128) ? 1 : 2;
     static constexpr int A_COLS = kOpRow / 4;
     static constexpr int A_BASE = ACC_BUFS * BN;
     static constexpr int TMEM_NEED = A_BASE + (TA ? NA * KB * A_COLS : 0);
     static constexpr int TMEM_COLS = TMEM_NEED <= 128 ? 128 : TMEM_NEED <= 256 ? 256 : 512;
     static_assert(TMEM_NEED <= 512, "tensor memory exceeded");
-    // Sets of four decode warps, one k-block of a stage each.  The integer pipe needs about 140 cycles for the codes of a
-    // k-block, a warp's round of waits and stores some 600 on top: tiles that do not hide that under their MMAs (four sets
-    // against two: 244 -> 185 ns per k-block of 64 rows) get four.
+    // Decode warps come in sets of four (one per lane quarter), a pair of sets takes a box of packed words: set i its k-blocks
+    // i and i + 2.  Everything a round does besides decoding (waits, addresses, arrivals: about 100 integer instructions
+    // against 72 for the codes of an int8 k-block) is paid once per box, and a second pair works on the next box meanwhile
+    // where the MMAs of a k-block do not cover the decoding of one.
     static constexpr int SETS = BN > 128 ? 2 : 4;
     static constexpr int DECODERS = DENSE ? 0 : 4 * SETS;
     static constexpr int FIRST_EPI = 4 + DECODERS;
     static constexpr int EPI = BN > 128 ? 8 : 4;                              // epilogue warps
-    static constexpr int READY = 4 * KB;                                    // warps that decode one stage
+    static constexpr int READY = KB == 1 ? 4 : 8;                             // warps that decode one stage
     static constexpr int THREADS = (FIRST_EPI + EPI) * 32;
     // shared memory
     static constexpr int A_OFF = 0;
@@ -102,69 +92,6 @@ struct ScaledCfg {
     static constexpr int bytes(int groups) { return TAB_OFF + 2 * 4 * (groups + 1) + 1024; }
     static_assert(TAB_OFF + 2 * 4 * (kMaxGroups + 1) + 1024 <= 227 * 1024, "shared memory exceeded");
 };
-
-// Unit u of the launch: rows [row0, row0 + rows) of group e, channels [n0, n0 + 128).
-struct Unit {
-    int e, row0, rows, n0;
-};
-// begin[e]: first row of group e, begin[groups]: end of the last; tiles[e]: row tiles before group e.  `e` only moves forward.
-__device__ __forceinline__ Unit locate(int u, int &e, const int *begin, const int *tiles, int tiles_n, int bn) {
-    const int rt = u / tiles_n;
-    while (tiles[e + 1] <= rt) e++;
-    Unit q;
-    q.e = e;
-    q.n0 = (u - rt * tiles_n) * kTileC;
-    q.row0 = begin[e] + (rt - tiles[e]) * bn;
-    const int left = begin[e + 1] - q.row0;
-    q.rows = left < bn ? left : bn;
-    return q;
-}
-
-// Executed by one warp: boundaries -> table.  Chunks of 32 boundaries, a running maximum and a running sum of tiles.
-__device__ __forceinline__ void build_table(const ScaledArgs &a, int *begin, int *tiles, int bn, int lane) {
-    if (!a.offsets) {
-        if (lane == 0) {
-            begin[0] = 0; begin[1] = (int)a.M;
-            tiles[0] = 0; tiles[1] = (int)((a.M + bn - 1) / bn);
-        }
-        return;
-    }
-    int run = 0, sum = 0;                                       // running maximum of the boundaries, tiles so far
-    for (int c = 0; c <= a.groups; c += 32) {
-        const int i = c + lane;
-        long long v = 0;
-        if (i <= a.groups)
-            v = a.offsets64 ? reinterpret_cast<const long long *>(a.offsets)[i] : reinterpret_cast<const int *>(a.offsets)[i];
-        int b = (int)(v < 0 ? 0 : v > a.M ? a.M : v);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, b, o);
-            if (lane >= o) b = max(b, x);
-        }
-        b = max(b, run);
-        int prev = __shfl_up_sync(0xffffffffu, b, 1);
-        if (lane == 0) prev = run;
-        int t = (i == 0 || i > a.groups) ? 0 : (b - prev + bn - 1) / bn;      // tiles of group i - 1
-        const int last = __shfl_sync(0xffffffffu, b, 31);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int x = __shfl_up_sync(0xffffffffu, t, o);
-            if (lane >= o) t += x;
-        }
-        if (i <= a.groups) {
-            begin[i] = b;
-            tiles[i] = sum + t;
-        }
-        sum += __shfl_sync(0xffffffffu, t, 31);
-        run = last;
-    }
-}
-
-__device__ __forceinline__ void store_one(void *Y, int y_type, long long i, float f) {
-    if (y_type == TMQ_TYPE_F32) reinterpret_cast<float *>(Y)[i] = f;
-    else if (y_type == TMQ_TYPE_BF16) reinterpret_cast<__nv_bfloat16 *>(Y)[i] = __float2bfloat16_rn(f);
-    else reinterpret_cast<__half *>(Y)[i] = __float2half_rn(f);
-}
 
 // One warp's 32 rows x 32 channels (f[j]: row j of this lane's channel) to Y.  TYPE fixed at compile time, addresses stepped.
 // FULL: all of them exist.  PAIRS: 16-bit results of two rows are paired between neighbouring lanes (even lanes keep row j,
@@ -246,7 +173,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         }
         for (int s = 0; s < C::RAW_STAGES; s++) {
             ptx::mbar_init(raw_full + s, 1);
-            ptx::mbar_init(raw_empty + s, C::DECODERS);
+            ptx::mbar_init(raw_empty + s, 8);
         }
         for (int b = 0; b < 2; b++) {
             ptx::mbar_init(acc_full + b, 1);
@@ -277,9 +204,9 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             uint32_t ph = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-                const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
-                const int rows = q.rows > C::BOX1 ? C::BOX0 : q.rows > C::BOX2 ? C::BOX1 : C::BOX2;
-                const CUtensorMap *mx = maps.x + (q.rows > C::BOX1 ? 0 : q.rows > C::BOX2 ? 1 : 2);
+                const Unit q = locate(u, e, begin, tiles, tiles_n, BN, kTileC);
+                const int box = q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2, rows = maps.height[box];
+                const CUtensorMap *mx = maps.x + box;
                 const int wrow = (int)(q.e * a.N) + q.n0;
                 const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : 0));      // of one k-block
                 for (int kb = 0; kb < nkb; kb += C::KB) {
@@ -314,9 +241,10 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             // even lanes watch the weights' barrier, odd lanes the activations': one round for both
             const bool acts = C::DENSE || (lane & 1);
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x, ti++) {
-                const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
+                const Unit q = locate(u, e, begin, tiles, tiles_n, BN, kTileC);
                 const uint32_t n_mma = (uint32_t)((q.rows + kRowStep - 1) / kRowStep * kRowStep);
-                const uint32_t b_step = (uint32_t)((q.rows > C::BOX1 ? C::BOX0 : q.rows > C::BOX2 ? C::BOX1 : C::BOX2) * kOpRow) >> 4;
+                const int height = maps.height[q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2];
+                const uint32_t b_step = (uint32_t)(height * kOpRow) >> 4;
                 const uint32_t idesc = ((C::I8 ? 2u : 1u) << 4) | (1u << 7) | (1u << 10) | ((n_mma >> 3) << 17) | ((128u >> 4) << 24);
                 const int buf = C::ACC_BUFS == 2 ? (ti & 1) : 0;
                 const uint32_t use = (uint32_t)(C::ACC_BUFS == 2 ? (ti >> 1) : ti);
@@ -375,7 +303,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             uint32_t ph = 1;
             bool ok = true;
             for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-                const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
+                const Unit q = locate(u, e, begin, tiles, tiles_n, BN, kTileC);
                 const int wrow = (int)(q.e * a.N) + q.n0;
                 for (int kb = 0; kb < nkb; kb += C::RAWK) {
                     ok = ptx::mbar_wait_idle(raw_empty + s, ph, a.status);
@@ -391,78 +319,91 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         }
     } else if (!C::DENSE && warp >= 4 && warp < C::FIRST_EPI) {
         // ---------------------------------------------------------------- decode
-        const int quarter = warp & 3, set = (warp - 4) >> 2;
+        const int quarter = warp & 3, pair = (warp - 4) >> 3, half = ((warp - 4) >> 2) & 1;
         const int row = quarter * 32 + lane;
+        const uint32_t raw_row = ptx::smem_u32(smem + C::RAW_OFF) + (uint32_t)(row * C::RAW_PITCH);
+        const uint32_t swz = (uint32_t)(C::RAW_PITCH == 128 ? row & 7 : (row >> 1) & 3) << 4;
+        const uint32_t a_row = ptx::smem_u32(smem + C::A_OFF) + (uint32_t)(row * kOpRow);
+        const uint32_t a_lane = tmem_base + ((uint32_t)(quarter * 32) << 16) + C::A_BASE;
+        const uint32_t ready0 = ptx::smem_u32(ready), taken0 = ptx::smem_u32(taken), raw_full0 = ptx::smem_u32(raw_full),
+                       raw_empty0 = ptx::smem_u32(raw_empty);
         bool ok = healthy;
-        int it = 0, s = 0, rs = 0;
-        uint32_t ph = 0, rph = 0;
+        int s = 0, rs = 0, turn = 0;
+        uint32_t ph = 1, rph = 0;                        // parities: slot taken by the MMAs, box landed
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-            for (int kb0 = 0; kb0 < nkb && ok; kb0 += C::RAWK) {
-                const uint8_t *raw = smem + C::RAW_OFF + rs * C::RAW_BYTES + row * C::RAW_PITCH;
-                bool seen = false;
-                for (int st = 0; st < C::RAWK && kb0 + st < nkb; st += C::KB) {
-                    // k-block j of stage it belongs to set (it KB + j) mod SETS
-                    const int j = (set - it * C::KB) & (C::SETS - 1);
-                    if (j < C::KB) {
-                    // even lanes wait for the packed words, odd lanes until the MMAs that read this stage last are done; a
-                    // set whose k-block lies beyond the unit waits (and reports) as well, or it would run a round ahead
-                    ok = ptx::mbar_wait_warp((lane & 1) ? taken + s : raw_full + rs, (lane & 1) ? ph ^ 1u : rph, a.status);
-                    if (!ok) break;
-                    seen = true;
-                    if (kb0 + st + j < nkb) {
-                        uint4 p[C::I8 ? 2 : 1];
+            for (int left = nkb; left > 0; left -= C::RAWK) {
+                if (C::SETS == 2 || turn == pair) {
 #pragma unroll
-                        for (int h = 0; h < (C::I8 ? 2 : 1); h++) {
-                            const int c = (C::I8 ? 2 * (st + j) : st + j) + h;
-                            p[h] = *reinterpret_cast<const uint4 *>(raw + ((c ^ (C::RAW_PITCH == 128 ? row & 7 : (row >> 1) & 3)) << 4));
+                    for (int st = 0; st < C::RAWK; st += C::KB) {
+                        if (st > 0 && st >= left) break;
+                        if (C::KB == 1 && st != half) {  // one k-block per stage: the other set's
+                            if (++s == C::NA) { s = 0; ph ^= 1u; }
+                            continue;
                         }
-                        uint32_t cols[32];                   // the row's 128 operand bytes, K ascending
-                        if (C::I8) {
-                            const uint32_t words[8] = {p[0].x, p[0].y, p[0].z, p[0].w, p[C::I8].x, p[C::I8].y, p[C::I8].z, p[C::I8].w};
+                        // even lanes wait for the packed words, odd lanes for the slot; a set whose k-block lies beyond the
+                        // unit waits (and reports) as well, or it would run a round ahead of the others
+                        ok = ptx::mbar_wait_warp_at((lane & 1) ? taken0 + 8u * s : raw_full0 + 8u * rs, (lane & 1) ? ph : rph, a.status);
+                        if (!ok) break;
+                        if (C::TA) ptx::tc_fence_after_sync();
 #pragma unroll
-                            for (int wi = 0; wi < 8; wi++) {
-                                uint32_t r[4];
-                                decode_word_i8_ptx(words[wi], r);
+                        for (int jj = 0; jj < (C::KB == 4 ? 2 : 1); jj++) {
+                            // k-block of the box, and of the stage
+                            const int j = C::KB == 4 ? half + 2 * jj : C::KB == 2 ? st + half : st, js = C::KB == 1 ? 0 : j - st;
+                            if (j > 0 && j >= left) break;
+                            const uint32_t words0 = raw_row + (uint32_t)(rs * C::RAW_BYTES);
+                            uint32_t cols[32];           // the row's 128 operand bytes, K ascending
+                            if (C::I8) {
+                                const uint4 p = ptx::lds_v4(words0 + (((uint32_t)(2 * j) << 4) ^ swz));
+                                const uint4 r = ptx::lds_v4(words0 + (((uint32_t)(2 * j + 1) << 4) ^ swz));
+                                const uint32_t words[8] = {p.x, p.y, p.z, p.w, r.x, r.y, r.z, r.w};
 #pragma unroll
-                                for (int x = 0; x < 4; x++) cols[4 * wi + x] = r[x];
+                                for (int wi = 0; wi < 8; wi++) {
+                                    uint32_t d[4];
+                                    decode_word_i8_ptx(words[wi], d);
+#pragma unroll
+                                    for (int x = 0; x < 4; x++) cols[4 * wi + x] = d[x];
+                                }
+                            } else {
+                                const uint4 p = ptx::lds_v4(words0 + (((uint32_t)j << 4) ^ swz));
+                                const uint32_t words[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                                for (int wi = 0; wi < 4; wi++) {
+                                    uint32_t d[8];
+                                    decode_word_bf16(words[wi], d);
+#pragma unroll
+                                    for (int x = 0; x < 8; x++) cols[8 * wi + x] = d[x];
+                                }
                             }
-                        } else {
-                            const uint32_t words[4] = {p[0].x, p[0].y, p[0].z, p[0].w};
+                            if (C::TA) {
+                                ptx::tmem_st_x32(a_lane + (uint32_t)((s * C::KB + js) * C::A_COLS), cols);
+                            } else {
+                                const uint32_t dst = a_row + (uint32_t)((s * C::KB + js) * C::A_BYTES);
 #pragma unroll
-                            for (int wi = 0; wi < 4; wi++) {
-                                uint32_t r[8];
-                                decode_word_bf16(words[wi], r);
-#pragma unroll
-                                for (int x = 0; x < 8; x++) cols[8 * wi + x] = r[x];
+                                for (int c = 0; c < 8; c++)
+                                    ptx::sts_v4(dst + (uint32_t)((c ^ (row & 7)) << 4), cols[4 * c], cols[4 * c + 1], cols[4 * c + 2],
+                                                cols[4 * c + 3]);
                             }
                         }
                         if (C::TA) {
-                            ptx::tc_fence_after_sync();
-                            ptx::tmem_st_x32(tmem_base + ((uint32_t)(quarter * 32) << 16) + C::A_BASE +
-                                                 (uint32_t)((s * C::KB + j) * C::A_COLS), cols);
+                            ptx::tmem_st_wait();
+                            ptx::tc_fence_before_sync();
                         } else {
-                            uint8_t *arow = smem + C::A_OFF + (s * C::KB + j) * C::A_BYTES + row * kOpRow;
-#pragma unroll
-                            for (int c = 0; c < 8; c++)
-                                *reinterpret_cast<uint4 *>(arow + ((c ^ (row & 7)) << 4)) =
-                                    make_uint4(cols[4 * c], cols[4 * c + 1], cols[4 * c + 2], cols[4 * c + 3]);
+                            ptx::fence_proxy_async_smem();
                         }
+                        __syncwarp();
+                        if (lane == 0) ptx::mbar_arrive_at(ready0 + 8u * s);
+                        if (++s == C::NA) { s = 0; ph ^= 1u; }
                     }
-                    if (C::TA) {
-                        ptx::tmem_st_wait();
-                        ptx::tc_fence_before_sync();
-                    } else {
-                        ptx::fence_proxy_async_smem();
-                    }
+                    if (!ok) break;
+                    if (C::KB == 1 && half == 1 && left == 1)        // no stage of its own in this box: wait for it all the same
+                        ok = ptx::mbar_wait_warp_at(raw_full0 + 8u * rs, rph, a.status);
                     __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(ready + s);
-                    }
-                    it++;
-                    if (++s == C::NA) { s = 0; ph ^= 1u; }
+                    if (ok && lane == 0) ptx::mbar_arrive_at(raw_empty0 + 8u * rs);
+                } else {                                 // the other pair's box
+                    s += left > C::RAWK - C::KB ? C::RAWK / C::KB : (left + C::KB - 1) / C::KB;
+                    if (s >= C::NA) { s -= C::NA; ph ^= 1u; }
                 }
-                if (ok && !seen) ok = ptx::mbar_wait_warp(raw_full + rs, rph, a.status);
-                __syncwarp();
-                if (ok && lane == 0) ptx::mbar_arrive(raw_empty + rs);
+                if (C::SETS == 4) turn ^= 1;
                 if (++rs == C::RAW_STAGES) { rs = 0; rph ^= 1u; }
             }
         }
@@ -476,7 +417,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         bool ok = healthy;
         int ti = 0, e = 0;
         for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x, ti++) {
-            const Unit q = locate(u, e, begin, tiles, tiles_n, BN);
+            const Unit q = locate(u, e, begin, tiles, tiles_n, BN, kTileC);
             const int n = q.n0 + quarter * 32 + lane;
             float sc = 1.0f, bi = 0.0f;
             if (n < a.N) {
@@ -526,15 +467,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                           : store_rows<TMQ_TYPE_F16, false>(Y, row, a.ldy, n, a.N, left, lane, f);
             }
         }
-        if (a.zero_rest && healthy) {
-            // rows before the first and behind the last group of a fresh result
-            const long long lead = begin[0], tail = begin[a.groups], total = lead + (a.M - tail);
-            for (long long r = blockIdx.x; r < total; r += gridDim.x) {
-                const long long m = r < lead ? r : tail + (r - lead);
-                for (long long n = threadIdx.x - C::FIRST_EPI * 32; n < a.N; n += C::EPI * 32)
-                    store_one(a.Y, a.y_type, m * a.ldy + n, 0.0f);
-            }
-        }
+        if (a.zero_rest && healthy) zero_rest_rows(a, begin, (int)threadIdx.x - C::FIRST_EPI * 32, C::EPI * 32);
     }
     ptx::tc_fence_before_sync();
     __syncthreads();
@@ -546,22 +479,21 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
 
 // ---- host side --------------------------------------------------------------------------------------------------------
 
-struct ScaledProblem {
-    const void *X, *W;
-    long long ldx, ldw;              // row strides of X (elements) and of 8-bit weights (bytes)
-    ScaledArgs a;
-};
-
 template <int WK, int BN>
 static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     using C = ScaledCfg<WK, BN>;
     ScaledArgs a = p.a;
     ScaledMaps maps;
     const CUtensorMapDataType xt = C::I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-    const int xe = C::I8 ? 1 : 2, box[3] = {C::BOX0, C::BOX1, C::BOX2};
+    const int xe = C::I8 ? 1 : 2;
+    const int last = (int)(a.M % BN + 7) / 8 * 8;         // rows of a plain product's last tile
+    maps.height[0] = BN;
+    maps.height[1] = a.groups > 1 ? BN / 2 : last ? last : BN;
+    maps.height[2] = a.groups > 1 ? BN / 4 : maps.height[1];
     a.wide = a.K % C::BK == 0;
     for (int i = 0; i < 3; i++)
-        if (!make_map_blocks(maps.x + i, xt, xe, p.X, (uint64_t)a.K, (uint64_t)a.M, (uint64_t)p.ldx * xe, C::BK, box[i], C::KB, a.wide))
+        if (!make_map_blocks(maps.x + i, xt, xe, p.X, (uint64_t)a.K, (uint64_t)a.M, (uint64_t)p.ldx * xe, C::BK, maps.height[i],
+                             C::KB, a.wide))
             return TMQ_ERR_LAUNCH;
     const uint64_t wrows = (uint64_t)a.groups * (uint64_t)a.N;
     const bool okw = C::DENSE
