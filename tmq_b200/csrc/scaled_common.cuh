@@ -30,22 +30,51 @@ struct ScaledProblem {
     ScaledArgs a;
 };
 
-int launch_scaled_skinny(int kind, const ScaledProblem &p, cudaStream_t st);
 
 #ifdef __CUDACC__
-// Unit u of the launch: rows [row0, row0 + rows) of group e, channels [n0, n0 + tile_c).
+// The units of a CTA: channel tile fastest, every gridDim.x-th unit.  A whole warp walks; per unit it costs two additions and,
+// for the expert, one look at 32 table entries (a division and a search by one thread took up to 2800 cycles beside busy
+// decode warps, more than the unit's k-blocks).
+struct Walk {
+    int rt, nt, e;                           // row tile, channel tile, expert
+    int d_rt, d_nt, tiles_n, total;
+    // begin[e]: first row of group e, begin[groups]: end of the last; tiles[e]: row tiles before group e
+    __device__ __forceinline__ Walk(const int *tiles, int groups, int tiles_n_) {
+        tiles_n = tiles_n_;
+        total = tiles[groups];
+        rt = (int)blockIdx.x / tiles_n;
+        nt = (int)blockIdx.x - rt * tiles_n;
+        d_rt = (int)gridDim.x / tiles_n;
+        d_nt = (int)gridDim.x - d_rt * tiles_n;
+        e = 0;
+    }
+    __device__ __forceinline__ bool more() const { return rt < total; }
+    __device__ __forceinline__ void next() {
+        rt += d_rt;
+        nt += d_nt;
+        if (nt >= tiles_n) {
+            nt -= tiles_n;
+            rt++;
+        }
+    }
+};
+
+// The unit a walk stands on: rows [row0, row0 + rows) of group e, channels [n0, n0 + tile_c).  Whole converged warp.
 struct Unit {
     int e, row0, rows, n0;
 };
-// begin[e]: first row of group e, begin[groups]: end of the last; tiles[e]: row tiles before group e.  `e` only moves forward.
-__device__ __forceinline__ Unit locate(int u, int &e, const int *begin, const int *tiles, int tiles_n, int bn, int tile_c) {
-    const int rt = u / tiles_n;
-    while (tiles[e + 1] <= rt) e++;
+__device__ __forceinline__ Unit locate(Walk &w, const int *begin, const int *tiles, int groups, int bn, int tile_c, int lane) {
+    for (;;) {                               // tiles[] does not decrease: the entries at or below rt are a prefix
+        const int i = w.e + 1 + lane;
+        const int n = __popc(__ballot_sync(0xffffffffu, i <= groups && tiles[i] <= w.rt));
+        w.e += n;
+        if (n < 32) break;
+    }
     Unit q;
-    q.e = e;
-    q.n0 = (u - rt * tiles_n) * tile_c;
-    q.row0 = begin[e] + (rt - tiles[e]) * bn;
-    const int left = begin[e + 1] - q.row0;
+    q.e = w.e;
+    q.n0 = w.nt * tile_c;
+    q.row0 = begin[w.e] + (w.rt - tiles[w.e]) * bn;
+    const int left = begin[w.e + 1] - q.row0;
     q.rows = left < bn ? left : bn;
     return q;
 }

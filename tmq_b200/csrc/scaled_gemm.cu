@@ -93,12 +93,12 @@ struct ScaledCfg {
     static_assert(TAB_OFF + 2 * 4 * (kMaxGroups + 1) + 1024 <= 227 * 1024, "shared memory exceeded");
 };
 
-// One warp's 32 rows x 32 channels (f[j]: row j of this lane's channel) to Y.  TYPE fixed at compile time, addresses stepped.
-// FULL: all of them exist.  PAIRS: 16-bit results of two rows are paired between neighbouring lanes (even lanes keep row j,
-// odd lanes row j + 1), so a warp writes 4 bytes a lane, two 64-byte runs; otherwise one row's 32 channels at a time.
-template <int TYPE, bool PAIRS, bool FULL>
+// One warp's COUNT rows x 32 channels (f[j]: row j of this lane's channel) to Y.  TYPE fixed at compile time, addresses
+// stepped.  FULL: all of them exist.  PAIRS: 16-bit results of two rows are paired between neighbouring lanes (even lanes keep
+// row j, odd lanes row j + 1), so a warp writes 4 bytes a lane, two 64-byte runs; otherwise one row's 32 channels at a time.
+template <int TYPE, bool PAIRS, bool FULL, int COUNT>
 __device__ __forceinline__ void store_rows(uint8_t *Y, long long row, long long ldy, int n, long long N, int left, int lane,
-                                           const float (&f)[32]) {
+                                           const float (&f)[COUNT]) {
     constexpr int ES = TYPE == TMQ_TYPE_F32 ? 4 : 2;
     const int odd = PAIRS ? lane & 1 : 0;
     const int nb = n - odd;
@@ -107,7 +107,7 @@ __device__ __forceinline__ void store_rows(uint8_t *Y, long long row, long long 
     const int rows = nb < N ? left - odd : 0;
     const bool both = nb + 1 < N;
 #pragma unroll
-    for (int j = 0; j < 32; j += (PAIRS ? 2 : 1)) {
+    for (int j = 0; j < COUNT; j += (PAIRS ? 2 : 1)) {
         if (PAIRS) {
             const float got = __shfl_xor_sync(0xffffffffu, odd ? f[j] : f[j + (PAIRS ? 1 : 0)], 1);
             const float lo = odd ? got : f[j], hi = odd ? f[j + (PAIRS ? 1 : 0)] : got;
@@ -131,11 +131,25 @@ __device__ __forceinline__ void store_rows(uint8_t *Y, long long row, long long 
     }
 }
 
-template <int TYPE, bool PAIRS>
-__device__ __forceinline__ void store_rows(uint8_t *Y, long long row, long long ldy, int n, long long N, int left, int lane,
-                                           const float (&f)[32]) {
-    if (left >= 32 && n - lane + 32 <= N) store_rows<TYPE, PAIRS, true>(Y, row, ldy, n, N, left, lane, f);
-    else store_rows<TYPE, PAIRS, false>(Y, row, ldy, n, N, left, lane, f);
+// COUNT accumulator columns (rows of the result) of this lane's channel -> results.  rs: their row scales, or null for 1.
+template <bool I8, int COUNT>
+__device__ __forceinline__ void finish_rows(const uint32_t (&v)[COUNT], const float *rs, float sc, float bi, const ScaledArgs &a,
+                                            bool pairs, long long row, int n, int left, int lane) {
+    float f[COUNT];
+#pragma unroll
+    for (int j = 0; j < COUNT; j++) {
+        const float acc = I8 ? __fmul_rn(__int2float_rn((int)v[j]), rs[j]) : __uint_as_float(v[j]);
+        f[j] = fmaf(acc, sc, bi);
+    }
+    uint8_t *Y = reinterpret_cast<uint8_t *>(a.Y);
+    const bool full = left >= COUNT && n - lane + 32 <= a.N;
+#define TMQ_STORE(TYPE, PAIRS)                                                                            \
+    (full ? store_rows<TYPE, PAIRS, true, COUNT>(Y, row, a.ldy, n, a.N, left, lane, f)                    \
+          : store_rows<TYPE, PAIRS, false, COUNT>(Y, row, a.ldy, n, a.N, left, lane, f))
+    if (a.y_type == TMQ_TYPE_F32) TMQ_STORE(TMQ_TYPE_F32, false);
+    else if (a.y_type == TMQ_TYPE_BF16) pairs ? TMQ_STORE(TMQ_TYPE_BF16, true) : TMQ_STORE(TMQ_TYPE_BF16, false);
+    else pairs ? TMQ_STORE(TMQ_TYPE_F16, true) : TMQ_STORE(TMQ_TYPE_F16, false);
+#undef TMQ_STORE
 }
 
 template <int WK, int BN>
@@ -195,35 +209,37 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
     const bool healthy = (*reinterpret_cast<volatile int *>(a.status) == 0);
-    const int nunits = tiles[a.groups] * tiles_n;
 
     if (warp == 0) {
-        // ---------------------------------------------------------------- TMA producer
-        if (lane == 0 && healthy) {
-            int s = 0, e = 0, round = 0;
+        // ---------------------------------------------------------------- TMA producer (whole warp walks, one lane issues)
+        if (healthy) {
+            int s = 0, round = 0;
             uint32_t ph = 1;
             bool ok = true;
-            for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-                const Unit q = locate(u, e, begin, tiles, tiles_n, BN, kTileC);
+            for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next()) {
+                const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
                 const int box = q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2, rows = maps.height[box];
                 const CUtensorMap *mx = maps.x + box;
                 const int wrow = (int)(q.e * a.N) + q.n0;
                 const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : 0));      // of one k-block
                 for (int kb = 0; kb < nkb; kb += C::KB) {
                     const int n = nkb - kb < C::KB ? nkb - kb : C::KB;
-                    ok = ptx::mbar_wait_idle(empty + s, ph, a.status);
+                    ok = __all_sync(0xffffffffu, ptx::mbar_wait_idle(empty + s, ph, a.status) ? 1 : 0) != 0;
                     if (!ok) break;
-                    uint8_t *wd = smem + C::A_OFF + s * C::KB * C::A_BYTES, *xd = smem + C::B_OFF + s * C::KB * C::B_BYTES;
-                    ptx::mbar_arrive_expect_tx(full + s, bytes * (uint32_t)(a.wide ? C::KB : n));
-                    if (a.wide) {                        // k-blocks beyond the row are filled with zeros, and counted
-                        if (C::DENSE) ptx::tma_load_3d(wd, &maps.w, full + s, 0, wrow, kb);
-                        ptx::tma_load_3d(xd, mx, full + s, 0, q.row0, kb);
-                    } else {
-                        for (int j = 0; j < n; j++) {
-                            if (C::DENSE) ptx::tma_load_3d(wd + j * C::A_BYTES, &maps.w, full + s, (kb + j) * C::BK, wrow, 0);
-                            ptx::tma_load_3d(xd + j * rows * kOpRow, mx, full + s, (kb + j) * C::BK, q.row0, 0);
+                    if (ptx::elect_one()) {
+                        uint8_t *wd = smem + C::A_OFF + s * C::KB * C::A_BYTES, *xd = smem + C::B_OFF + s * C::KB * C::B_BYTES;
+                        ptx::mbar_arrive_expect_tx(full + s, bytes * (uint32_t)(a.wide ? C::KB : n));
+                        if (a.wide) {                    // k-blocks beyond the row are filled with zeros, and counted
+                            if (C::DENSE) ptx::tma_load_3d(wd, &maps.w, full + s, 0, wrow, kb);
+                            ptx::tma_load_3d(xd, mx, full + s, 0, q.row0, kb);
+                        } else {
+                            for (int j = 0; j < n; j++) {
+                                if (C::DENSE) ptx::tma_load_3d(wd + j * C::A_BYTES, &maps.w, full + s, (kb + j) * C::BK, wrow, 0);
+                                ptx::tma_load_3d(xd + j * rows * kOpRow, mx, full + s, (kb + j) * C::BK, q.row0, 0);
+                            }
                         }
                     }
+                    __syncwarp();
                     if (++s == C::NB) { s = 0; ph ^= 1u; round = 1; }
                 }
             }
@@ -235,13 +251,13 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (whole warp walks, one lane issues)
         if (healthy) {
-            int sa = 0, sb = 0, ti = 0, e = 0;
+            int sa = 0, sb = 0, ti = 0;
             uint32_t pa = 0, pb = 0;
             bool ok = true, landed = false;
             // even lanes watch the weights' barrier, odd lanes the activations': one round for both
             const bool acts = C::DENSE || (lane & 1);
-            for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x, ti++) {
-                const Unit q = locate(u, e, begin, tiles, tiles_n, BN, kTileC);
+            for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next(), ti++) {
+                const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
                 const uint32_t n_mma = (uint32_t)((q.rows + kRowStep - 1) / kRowStep * kRowStep);
                 const int height = maps.height[q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2];
                 const uint32_t b_step = (uint32_t)(height * kOpRow) >> 4;
@@ -298,18 +314,21 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         }
     } else if (warp == 2) {
         // ---------------------------------------------------------------- TMA producer of the packed words
-        if (!C::DENSE && lane == 0 && healthy) {
-            int s = 0, e = 0, round = 0;
+        if (!C::DENSE && healthy) {
+            int s = 0, round = 0;
             uint32_t ph = 1;
             bool ok = true;
-            for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
-                const Unit q = locate(u, e, begin, tiles, tiles_n, BN, kTileC);
+            for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next()) {
+                const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
                 const int wrow = (int)(q.e * a.N) + q.n0;
                 for (int kb = 0; kb < nkb; kb += C::RAWK) {
-                    ok = ptx::mbar_wait_idle(raw_empty + s, ph, a.status);
+                    ok = __all_sync(0xffffffffu, ptx::mbar_wait_idle(raw_empty + s, ph, a.status) ? 1 : 0) != 0;
                     if (!ok) break;
-                    ptx::mbar_arrive_expect_tx(raw_full + s, (uint32_t)C::RAW_BYTES);
-                    ptx::tma_load_2d(smem + C::RAW_OFF + s * C::RAW_BYTES, &maps.w, raw_full + s, kb * (C::RAW_ROW / 4), wrow);
+                    if (ptx::elect_one()) {
+                        ptx::mbar_arrive_expect_tx(raw_full + s, (uint32_t)C::RAW_BYTES);
+                        ptx::tma_load_2d(smem + C::RAW_OFF + s * C::RAW_BYTES, &maps.w, raw_full + s, kb * (C::RAW_ROW / 4), wrow);
+                    }
+                    __syncwarp();
                     if (++s == C::RAW_STAGES) { s = 0; ph ^= 1u; round = 1; }
                 }
             }
@@ -330,7 +349,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         bool ok = healthy;
         int s = 0, rs = 0, turn = 0;
         uint32_t ph = 1, rph = 0;                        // parities: slot taken by the MMAs, box landed
-        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x) {
+        for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next()) {
             for (int left = nkb; left > 0; left -= C::RAWK) {
                 if (C::SETS == 2 || turn == pair) {
 #pragma unroll
@@ -409,62 +428,62 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         }
     } else if (warp >= C::FIRST_EPI) {
         // ---------------------------------------------------------------- epilogue
-        // lane = channel, accumulator column = row: 32 rows at a time
+        // lane = channel, accumulator column = row: 32 rows at a time, what is left of a unit 8 at a time
         const int quarter = warp & 3, group = (warp - C::FIRST_EPI) >> 2;
         constexpr int kStep = 8 * C::EPI;                 // rows the epilogue warps of a quarter take per round
         float *rs = reinterpret_cast<float *>(smem + C::RS_OFF) + (warp - C::FIRST_EPI) * 32;
         const bool pairs = a.y_type != TMQ_TYPE_F32 && (a.ldy & 1) == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 3) == 0;
         bool ok = healthy;
-        int ti = 0, e = 0;
-        for (int u = blockIdx.x; u < nunits && ok; u += gridDim.x, ti++) {
-            const Unit q = locate(u, e, begin, tiles, tiles_n, BN, kTileC);
+        int ti = 0;
+        for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next(), ti++) {
+            const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
             const int n = q.n0 + quarter * 32 + lane;
-            float sc = 1.0f, bi = 0.0f;
+            float sc = 1.0f, bi = 0.0f, r = 1.0f;
             if (n < a.N) {
                 if (a.scale) sc = a.scale[(long long)q.e * a.N + n];
                 if (a.bias) bi = a.bias[(long long)q.e * a.N + n];
             }
             if (!C::I8) sc *= 0.5f;                      // bf16 weights are carried as +-2
+            int c = 32 * group;
+            if (C::I8 && a.row_scale && c + lane < q.rows) r = a.row_scale[q.row0 + c + lane];
             const int buf = C::ACC_BUFS == 2 ? (ti & 1) : 0;
             ok = ptx::mbar_wait_idle(acc_full + buf, (uint32_t)(C::ACC_BUFS == 2 ? (ti >> 1) : ti) & 1u, a.status);
             ok = __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
             if (!ok) break;
             ptx::tc_fence_after_sync();
             const uint32_t lane_addr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(buf * BN);
+            auto release = [&]() {                       // everything read: the accumulator goes back to the MMA warp
+                ptx::tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) ptx::mbar_arrive(acc_empty + buf);
+            };
+            if (c >= q.rows) release();
 #pragma unroll 1
-            for (int c = 32 * group; c < q.rows + kStep; c += kStep) {
-                if (c >= q.rows) {                       // nothing (more) to read: the accumulator goes back to the MMA warp
-                    ptx::tc_fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) ptx::mbar_arrive(acc_empty + buf);
-                    break;
-                }
-                uint32_t v[32];
-                ptx::tmem_ld_x16(lane_addr + (uint32_t)c, reinterpret_cast<uint32_t(&)[16]>(v[0]));
-                ptx::tmem_ld_x16(lane_addr + (uint32_t)c + 16, reinterpret_cast<uint32_t(&)[16]>(v[16]));
+            for (; c < q.rows; c += kStep) {
+                const int left = q.rows - c;
                 if (C::I8) {
-                    const float r = (a.row_scale && c + lane < q.rows) ? a.row_scale[q.row0 + c + lane] : 1.0f;
                     __syncwarp();
                     rs[lane] = r;
                     __syncwarp();
+                    if (a.row_scale && c + kStep + lane < q.rows) r = a.row_scale[q.row0 + c + kStep + lane];
                 }
-                ptx::tmem_ld_wait();
-                const int left = q.rows - c;
-                float f[32];
-#pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const float acc = C::I8 ? __fmul_rn(__int2float_rn((int)v[j]), rs[j]) : __uint_as_float(v[j]);
-                    f[j] = fmaf(acc, sc, bi);
+                if (left >= 32) {
+                    uint32_t v[32];
+                    ptx::tmem_ld_x16(lane_addr + (uint32_t)c, reinterpret_cast<uint32_t(&)[16]>(v[0]));
+                    ptx::tmem_ld_x16(lane_addr + (uint32_t)c + 16, reinterpret_cast<uint32_t(&)[16]>(v[16]));
+                    ptx::tmem_ld_wait();
+                    if (left <= kStep) release();
+                    finish_rows<C::I8, 32>(v, rs, sc, bi, a, pairs, q.row0 + c, n, left, lane);
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < left; j += 8) {
+                        uint32_t v[8];
+                        ptx::tmem_ld_x8(lane_addr + (uint32_t)(c + j), v);
+                        ptx::tmem_ld_wait();
+                        if (left - j <= 8) release();
+                        finish_rows<C::I8, 8>(v, rs + j, sc, bi, a, pairs, q.row0 + c + j, n, left - j, lane);
+                    }
                 }
-                uint8_t *Y = reinterpret_cast<uint8_t *>(a.Y);
-                const long long row = q.row0 + c;
-                if (a.y_type == TMQ_TYPE_F32) store_rows<TMQ_TYPE_F32, false>(Y, row, a.ldy, n, a.N, left, lane, f);
-                else if (a.y_type == TMQ_TYPE_BF16)
-                    pairs ? store_rows<TMQ_TYPE_BF16, true>(Y, row, a.ldy, n, a.N, left, lane, f)
-                          : store_rows<TMQ_TYPE_BF16, false>(Y, row, a.ldy, n, a.N, left, lane, f);
-                else
-                    pairs ? store_rows<TMQ_TYPE_F16, true>(Y, row, a.ldy, n, a.N, left, lane, f)
-                          : store_rows<TMQ_TYPE_F16, false>(Y, row, a.ldy, n, a.N, left, lane, f);
             }
         }
         if (a.zero_rest && healthy) zero_rest_rows(a, begin, (int)threadIdx.x - C::FIRST_EPI * 32, C::EPI * 32);
@@ -535,7 +554,7 @@ static int check_scaled(const ScaledProblem &p, int x_bytes, bool dense) {
     if (a.y_type < TMQ_TYPE_F32 || a.y_type > TMQ_TYPE_F16) return TMQ_ERR_ARG;
     if (a.M == 0) return TMQ_OK;
     if (!p.X || !p.W || !a.Y || !a.status || (dense && p.ldw < a.K)) return TMQ_ERR_ARG;
-    if (a.M > 0x7FFFFFFF || a.K > 0x7FFFFFFF || a.groups > kMaxGroups || a.N * a.groups > 0x7FFFFFFF) return TMQ_ERR_UNSUPPORTED;
+    if (a.M > 0x7FFFFF00 || a.K > 0x7FFFFFFF || a.groups > kMaxGroups || a.N * a.groups > 0x7FFFFFFF) return TMQ_ERR_UNSUPPORTED;
     // int32 sums of 8-bit products stay exact up to 2^31 / 2^14 of them
     if (x_bytes == 1 && a.K > 131071) return TMQ_ERR_UNSUPPORTED;
     if ((p.ldx * x_bytes) % 16 != 0 || (dense && p.ldw % 16 != 0)) return TMQ_ERR_UNSUPPORTED;

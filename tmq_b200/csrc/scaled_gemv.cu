@@ -44,7 +44,7 @@ __device__ __forceinline__ void store_result(void *Y, int y_type, long long i, f
 // Rows of X -> codes in shared memory (zero from K to the row pitch) and their scales.  16 / MP warps share a row.
 template <typename T, int MP>
 __device__ __forceinline__ void quantize_to_smem(const ScaledGemvArgs &a, uint8_t *xq, float *row_scale, uint32_t *red) {
-    constexpr int WPR = kSgWarps / MP, V = QuantType<T>::V, STEP = WPR * 32 * V, CH = 4;
+    constexpr int WPR = kSgWarps / MP, V = QuantType<T>::V, STEP = WPR * 32 * V, CH = MP == 8 ? 8 : 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int m = warp / WPR, t = (warp % WPR) * 32 + lane;
     const bool live = m < a.M;
