@@ -20,6 +20,7 @@ struct ScaledArgs {
     long long M, N, K, ldy;
     int groups, offsets64, y_type, zero_rest;
     int wide;                        // K is whole k-blocks: one box per stage
+    int rows_first;                  // order of the work units (plain product only)
     int *status;
 };
 
@@ -32,29 +33,36 @@ struct ScaledProblem {
 
 
 #ifdef __CUDACC__
-// The units of a CTA: channel tile fastest, every gridDim.x-th unit.  A whole warp walks; per unit it costs two additions and,
-// for the expert, one look at 32 table entries (a division and a search by one thread took up to 2800 cycles beside busy
-// decode warps, more than the unit's k-blocks).
+// The units of a CTA, every gridDim.x-th.  A whole warp walks; per unit it costs two additions and, for the expert, one look at
+// 32 table entries (a division and a search by one thread took up to 2800 cycles beside busy decode warps, more than the
+// unit's k-blocks).  Channel tiles run fastest, or row tiles (rows_first) where the weights are the larger operand: they are
+// then read from memory once and the activations stay in L2.
 struct Walk {
     int rt, nt, e;                           // row tile, channel tile, expert
-    int d_rt, d_nt, tiles_n, total;
+    int d_major, d_minor, minors, majors;
+    bool rows_first;
     // begin[e]: first row of group e, begin[groups]: end of the last; tiles[e]: row tiles before group e
-    __device__ __forceinline__ Walk(const int *tiles, int groups, int tiles_n_) {
-        tiles_n = tiles_n_;
-        total = tiles[groups];
-        rt = (int)blockIdx.x / tiles_n;
-        nt = (int)blockIdx.x - rt * tiles_n;
-        d_rt = (int)gridDim.x / tiles_n;
-        d_nt = (int)gridDim.x - d_rt * tiles_n;
+    __device__ __forceinline__ Walk(const int *tiles, const ScaledArgs &a, int tiles_n) {
+        rows_first = a.rows_first != 0;
+        const int total = tiles[a.groups];
+        minors = rows_first ? total : tiles_n;
+        majors = rows_first ? tiles_n : total;
+        const int first = minors > 0 ? (int)blockIdx.x / minors : 0;
+        d_major = minors > 0 ? (int)gridDim.x / minors : 0;
+        d_minor = (int)gridDim.x - d_major * minors;
+        const int minor = (int)blockIdx.x - first * minors;
+        rt = rows_first ? minor : first;
+        nt = rows_first ? first : minor;
         e = 0;
     }
-    __device__ __forceinline__ bool more() const { return rt < total; }
+    __device__ __forceinline__ bool more() const { return minors > 0 && (rows_first ? nt : rt) < majors; }
     __device__ __forceinline__ void next() {
-        rt += d_rt;
-        nt += d_nt;
-        if (nt >= tiles_n) {
-            nt -= tiles_n;
-            rt++;
+        int &minor = rows_first ? rt : nt, &major = rows_first ? nt : rt;
+        major += d_major;
+        minor += d_minor;
+        if (minor >= minors) {
+            minor -= minors;
+            major++;
         }
     }
 };

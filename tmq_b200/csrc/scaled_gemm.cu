@@ -216,7 +216,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             int s = 0, round = 0;
             uint32_t ph = 1;
             bool ok = true;
-            for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next()) {
+            for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next()) {
                 const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
                 const int box = q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2, rows = maps.height[box];
                 const CUtensorMap *mx = maps.x + box;
@@ -256,7 +256,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             bool ok = true, landed = false;
             // even lanes watch the weights' barrier, odd lanes the activations': one round for both
             const bool acts = C::DENSE || (lane & 1);
-            for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next(), ti++) {
+            for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next(), ti++) {
                 const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
                 const uint32_t n_mma = (uint32_t)((q.rows + kRowStep - 1) / kRowStep * kRowStep);
                 const int height = maps.height[q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2];
@@ -318,7 +318,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             int s = 0, round = 0;
             uint32_t ph = 1;
             bool ok = true;
-            for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next()) {
+            for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next()) {
                 const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
                 const int wrow = (int)(q.e * a.N) + q.n0;
                 for (int kb = 0; kb < nkb; kb += C::RAWK) {
@@ -349,7 +349,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         bool ok = healthy;
         int s = 0, rs = 0, turn = 0;
         uint32_t ph = 1, rph = 0;                        // parities: slot taken by the MMAs, box landed
-        for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next()) {
+        for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next()) {
             for (int left = nkb; left > 0; left -= C::RAWK) {
                 if (C::SETS == 2 || turn == pair) {
 #pragma unroll
@@ -435,7 +435,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         const bool pairs = a.y_type != TMQ_TYPE_F32 && (a.ldy & 1) == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 3) == 0;
         bool ok = healthy;
         int ti = 0;
-        for (Walk w(tiles, a.groups, tiles_n); w.more() && ok; w.next(), ti++) {
+        for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next(), ti++) {
             const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
             const int n = q.n0 + quarter * 32 + lane;
             float sc = 1.0f, bi = 0.0f, r = 1.0f;
@@ -510,6 +510,8 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     maps.height[1] = a.groups > 1 ? BN / 2 : last ? last : BN;
     maps.height[2] = a.groups > 1 ? BN / 4 : maps.height[1];
     a.wide = a.K % C::BK == 0;
+    const long long w_bytes = a.N * (C::DENSE ? p.ldw : prepack_row_words(a.K, C::I8 ? 1 : 0) * 4);
+    a.rows_first = a.groups == 1 && !a.offsets && w_bytes > a.M * p.ldx * xe;
     for (int i = 0; i < 3; i++)
         if (!make_map_blocks(maps.x + i, xt, xe, p.X, (uint64_t)a.K, (uint64_t)a.M, (uint64_t)p.ldx * xe, C::BK, maps.height[i],
                              C::KB, a.wide))
@@ -539,13 +541,45 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     return cuda_status(cudaLaunchKernelEx(&cfg, scaled_gemm_kernel<WK, BN>, maps, a));
 }
 
+// Rows of a work unit.  Tall tiles use each decoded weight and each copied byte for more rows, low ones leave more units for
+// the SMs and cost less to fill and drain.  Time = base + waves of units * k-blocks * ns per k-block, with what full tiles
+// measured: 155 / 160 / 240 / 352 ns for 32 / 64 / 128 / 256 rows (int8 and bf16 alike within a sixth), 0.6 us more to fill and
+// drain per doubling.  The row tiles of experts are not known here: the even share plus 0.6 of a tile each.  Over 150 shapes
+// (48 .. 2048 rows, 1 .. 128 experts with 1 .. 512 rows each on average) the choice costs 1 % on average against the best
+// tile of each; e.g. 517 x 11008 x 4096 int8 52.6 / 35.3 / 27.9 / 30.5 us, 64 experts of 48 rows 58.6 / 45.1 / 47.9 / 68.0 us,
+// of 512 rows 438 / 250 / 202 / 184 us.
+static int unit_rows(const ScaledArgs &a, int bk) {
+    static const double per_block[4] = {0.155, 0.160, 0.240, 0.352};
+    const double blocks = (double)((a.K + bk - 1) / bk), tiles_n = (double)((a.N + kTileC - 1) / kTileC);
+    int best = 32;
+    double best_cost = 0.0;
+    for (int i = 0, bn = 32; i < 4; i++, bn *= 2) {
+        double waves;
+        if (a.groups == 1) {
+            const long long units = (a.M + bn - 1) / bn * ((a.N + kTileC - 1) / kTileC);
+            waves = (double)((units + kNumSMs - 1) / kNumSMs);
+        } else {
+            const double partial = 0.6 * (double)(a.groups < a.M ? a.groups : a.M);
+            waves = ((double)a.M / bn + partial) * tiles_n / kNumSMs;
+            if (waves < 1.0) waves = 1.0;
+        }
+        const double cost = 0.6 * i + waves * blocks * per_block[i];
+        if (i == 0 || cost < best_cost) {
+            best = bn;
+            best_cost = cost;
+        }
+    }
+    return best;
+}
+
 template <int WK>
 static int dispatch_scaled(const ScaledProblem &p, cudaStream_t st) {
-    const long long per_group = (p.a.M + p.a.groups - 1) / p.a.groups;
-    if (per_group > 128) return launch_scaled<WK, 256>(p, st);
-    if (per_group > 64) return launch_scaled<WK, 128>(p, st);
-    if (per_group > 32) return launch_scaled<WK, 64>(p, st);
-    return launch_scaled<WK, 32>(p, st);
+    switch (unit_rows(p.a, WK == W_TERNARY_BF16 ? 64 : 128)) {
+        case 256: return launch_scaled<WK, 256>(p, st);
+        case 128: return launch_scaled<WK, 128>(p, st);
+        case 64: return launch_scaled<WK, 64>(p, st);
+        default: return launch_scaled<WK, 32>(p, st);
+    }
 }
 
 static int check_scaled(const ScaledProblem &p, int x_bytes, bool dense) {
@@ -571,7 +605,7 @@ using namespace tmq;
 extern "C" int tmq_ternary_gemm_a8(const int8_t *X, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
                                    const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy,
                                    int *status, void *stream) {
-    const ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, status}};
+    const ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, status}};
     const int rc = check_scaled(p, 1, false);
     if (rc != TMQ_OK || M == 0) return rc;
     return dispatch_scaled<W_TERNARY_I8>(p, (cudaStream_t)stream);
@@ -580,7 +614,7 @@ extern "C" int tmq_ternary_gemm_a8(const int8_t *X, int64_t ldx, const float *ro
 extern "C" int tmq_gemm_i8(const int8_t *X, int64_t ldx, const float *row_scale, const int8_t *W, int64_t ldw,
                            const float *scale, const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K,
                            int64_t ldy, int *status, void *stream) {
-    const ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, status}};
+    const ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, status}};
     const int rc = check_scaled(p, 1, true);
     if (rc != TMQ_OK || M == 0) return rc;
     return dispatch_scaled<W_DENSE_I8>(p, (cudaStream_t)stream);
@@ -591,7 +625,7 @@ extern "C" int tmq_ternary_gemm_grouped_bf16(const void *X, int64_t ldx, const u
                                              int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest,
                                              int *status, void *stream) {
     const ScaledProblem p = {X, Wt, ldx, 0,
-                             {nullptr, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, status}};
+                             {nullptr, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 2, false);
     if (rc != TMQ_OK || M == 0) return rc;
@@ -604,7 +638,7 @@ extern "C" int tmq_ternary_gemm_grouped_a8(const int8_t *X, int64_t ldx, const f
                                            int groups, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy,
                                            int zero_rest, int *status, void *stream) {
     const ScaledProblem p = {X, Wt, ldx, 0,
-                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, status}};
+                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 1, false);
     if (rc != TMQ_OK || M == 0) return rc;
@@ -617,7 +651,7 @@ extern "C" int tmq_gemm_grouped_i8(const int8_t *X, int64_t ldx, const float *ro
                                    void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest,
                                    int *status, void *stream) {
     const ScaledProblem p = {X, W, ldx, ldw,
-                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, status}};
+                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 1, true);
     if (rc != TMQ_OK || M == 0) return rc;
