@@ -262,29 +262,28 @@ int tmq_ternary_gemv_batched_i8(const int8_t *X, int64_t x_stride, const uint32_
 int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *scale, int64_t M, int64_t K, int64_t ldx, int64_t ldq,
                       int64_t cols, void *stream);
 
-/* Y[m][n] = acc * row_scale[m] * scale[n] + bias[n],  acc = sum_k X[m][k] W[n][k] exact in int32 (K <= 131071), then fp32:
+/* Y[m][n] = acc * row_scale[m] * scale[n] + bias[n],  acc = sum_k q[m][k] W[n][k] exact in int32 (K <= 131071), then fp32:
  * (acc * row_scale) rounded, times scale plus bias in one fused multiply-add, rounded once more to y_type (TMQ_TYPE_*).
- * row_scale [M], scale [N], bias [N]: fp32, NULL for 1 / 1 / 0.  X int8 [M][ldx], 16-byte aligned, ldx % 16 == 0, any
- * K <= ldx (columns beyond K are not used).  Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw],
- * 16-byte aligned, ldw % 16 == 0.  Y [M][ldy], element-aligned.
- * *status: see "Status word" above.
- * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549, and the post_scale / bias of Linear.compact_forward, tmq/tmq.py:662-688. */
-int tmq_ternary_gemm_a8(const int8_t *X, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
-                        const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
-                        void *stream);
-int tmq_gemm_i8(const int8_t *X, int64_t ldx, const float *row_scale, const int8_t *W, int64_t ldw, const float *scale,
-                const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
-                void *stream);
-
-/* tmq_ternary_gemm_a8 for one to eight rows, quantisation included, in one launch: X of x_type TMQ_TYPE_* (quantised as
- * tmq_quantize_rows does; any alignment; row_scale NULL) or x_type -1: int8 codes (16-byte aligned rows, ldx % 16 == 0) with
- * row_scale.  Same results, bit for bit.  TMQ_ERR_UNSUPPORTED when an SM's share of the matrix exceeds its shared memory
- * (N > 11840, or long rows): then quantise and call tmq_ternary_gemm_a8.  Wt is fetched ahead of the stream's previous kernel:
- * the CONTRACT of tmq_ternary_gemv_bf16 holds (scale, bias, row_scale and X carry no such restriction).
- * replaces: ternary_mvm_cuda, tmq/tmq_cuda.cu:563-603 (fp32 activations on CUDA cores). */
-int tmq_ternary_gemv_a8(const void *X, int x_type, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
-                        const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
-                        void *stream);
+ * scale [N], bias [N]: fp32, NULL for 1 / 0.
+ * x_type -1: X holds the codes, int8 [M][ldx], 16-byte aligned, ldx % 16 == 0, any K <= ldx (columns beyond K are not used),
+ *   row_scale fp32 [M] or NULL for 1.
+ * x_type TMQ_TYPE_*: X holds floating point [M][ldx] (element-aligned) and is quantised first, exactly as tmq_quantize_rows
+ *   does; row_scale NULL; workspace: tmq_a8_workspace_bytes(x_type, M, K) bytes of device scratch, 16-byte aligned
+ *   (TMQ_ERR_SCRATCH without it, before anything is launched).  tmq_ternary_gemm_a8 needs none for M <= 8 where an SM's share
+ *   of the matrix fits its shared memory (N <= 11840 and rows of a few thousand): quantisation and product are then one launch.
+ * Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw], 16-byte aligned, ldw % 16 == 0.
+ * Y [M][ldy], element-aligned.  *status: see "Status word" above.
+ * tmq_ternary_gemm_a8 with M <= 8 fetches Wt ahead of the stream's previous kernel: the CONTRACT of tmq_ternary_gemv_bf16 holds
+ * for Wt (not for scale, bias, row_scale, X).
+ * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549, ternary_mvm_cuda, :563-603, and the post_scale / bias of
+ * Linear.compact_forward, tmq/tmq.py:662-688 (fp32 activations on CUDA cores). */
+size_t tmq_a8_workspace_bytes(int x_type, int64_t M, int64_t K);
+int tmq_ternary_gemm_a8(const void *X, int x_type, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
+                        const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, void *workspace,
+                        size_t workspace_bytes, int *status, void *stream);
+int tmq_gemm_i8(const void *X, int x_type, int64_t ldx, const float *row_scale, const int8_t *W, int64_t ldw, const float *scale,
+                const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, void *workspace,
+                size_t workspace_bytes, int *status, void *stream);
 
 /* Products grouped by expert: rows offsets[e] .. offsets[e + 1] - 1 of X use matrix e of the stacked weights
  * ([groups][N] rows, the layouts above; bf16: tmq_prepack fmt 0, X bf16 with ldx % 8 == 0), scale and bias [groups][N].

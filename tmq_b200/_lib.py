@@ -94,10 +94,11 @@ _SIGNATURES = {
     "tmq_avgpool_nhwc_bf16": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "tmq_conv_patches_bf16": (c_int, [c_void_p, c_void_p] + [c_int] * 13 + [c_void_p]),
     "tmq_quantize_rows": (c_int, [c_void_p, c_int, c_void_p, c_void_p] + [c_int64] * 5 + [c_void_p]),
-    "tmq_ternary_gemm_a8": (c_int, [c_void_p, c_int64] + [c_void_p] * 5 + [c_int] + [c_int64] * 4 + [c_void_p, c_void_p]),
-    "tmq_ternary_gemv_a8": (c_int, [c_void_p, c_int, c_int64] + [c_void_p] * 5 + [c_int] + [c_int64] * 4 + [c_void_p, c_void_p]),
-    "tmq_gemm_i8": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 3 + [c_int] + [c_int64] * 4
-                    + [c_void_p, c_void_p]),
+    "tmq_a8_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64]),
+    "tmq_ternary_gemm_a8": (c_int, [c_void_p, c_int, c_int64] + [c_void_p] * 5 + [c_int] + [c_int64] * 4
+                            + [c_void_p, c_size_t, c_void_p, c_void_p]),
+    "tmq_gemm_i8": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64] + [c_void_p] * 3 + [c_int] + [c_int64] * 4
+                    + [c_void_p, c_size_t, c_void_p, c_void_p]),
     "tmq_ternary_gemm_grouped_bf16": (c_int, [c_void_p, c_int64] + [c_void_p] * 4 + [c_int, c_int, c_void_p, c_int]
                                       + [c_int64] * 4 + [c_int, c_void_p, c_void_p]),
     "tmq_ternary_gemm_grouped_a8": (c_int, [c_void_p, c_int64] + [c_void_p] * 5 + [c_int, c_int, c_void_p, c_int]

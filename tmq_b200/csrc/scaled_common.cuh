@@ -32,6 +32,12 @@ struct ScaledProblem {
 };
 
 
+// One to eight rows times a packed ternary matrix in one launch (scaled_gemv.cu); TMQ_ERR_UNSUPPORTED where an SM's share of
+// the matrix exceeds its shared memory.
+int launch_token_product(const void *X, int x_type, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
+                         const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
+                         cudaStream_t stream);
+
 #ifdef __CUDACC__
 // The units of a CTA, every gridDim.x-th.  A whole warp walks; per unit it costs two additions and, for the expert, one look at
 // 32 table entries (a division and a search by one thread took up to 2800 cycles beside busy decode warps, more than the

@@ -15,6 +15,7 @@
 #include "decode.cuh"
 #include "ptx.cuh"
 #include "quantize.cuh"
+#include "scaled_common.cuh"
 
 namespace tmq {
 
@@ -271,13 +272,9 @@ static int launch_scaled_gemv(const ScaledGemvArgs &a, unsigned grid, size_t sme
     return launch_chained(scaled_gemv_kernel<MP>, a, grid, kSgWarps * 32, smem, st);
 }
 
-}  // namespace tmq
-
-using namespace tmq;
-
-extern "C" int tmq_ternary_gemv_a8(const void *X, int x_type, int64_t ldx, const float *row_scale, const uint32_t *Wt,
-                                   const float *scale, const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K,
-                                   int64_t ldy, int *status, void *stream) {
+int launch_token_product(const void *X, int x_type, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
+                         const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int *status,
+                         cudaStream_t stream) {
     if (M < 0 || N <= 0 || K <= 0 || ldx < K || ldy < N || x_type < -1 || x_type > TMQ_TYPE_F16 || y_type < TMQ_TYPE_F32 ||
         y_type > TMQ_TYPE_F16 || (x_type >= 0 && row_scale))
         return TMQ_ERR_ARG;
@@ -301,8 +298,10 @@ extern "C" int tmq_ternary_gemv_a8(const void *X, int x_type, int64_t ldx, const
     a.x_offset = (int)((rows + 127) / 128 * 128);
     const long long smem = a.x_offset + M * a.x_pitch;
     if (smem > kSgSmemMax) return TMQ_ERR_UNSUPPORTED;
-    if (M == 1) return launch_scaled_gemv<1>(a, (unsigned)grid, (size_t)smem, (cudaStream_t)stream);
-    if (M == 2) return launch_scaled_gemv<2>(a, (unsigned)grid, (size_t)smem, (cudaStream_t)stream);
-    if (M <= 4) return launch_scaled_gemv<4>(a, (unsigned)grid, (size_t)smem, (cudaStream_t)stream);
-    return launch_scaled_gemv<8>(a, (unsigned)grid, (size_t)smem, (cudaStream_t)stream);
+    if (M == 1) return launch_scaled_gemv<1>(a, (unsigned)grid, (size_t)smem, stream);
+    if (M == 2) return launch_scaled_gemv<2>(a, (unsigned)grid, (size_t)smem, stream);
+    if (M <= 4) return launch_scaled_gemv<4>(a, (unsigned)grid, (size_t)smem, stream);
+    return launch_scaled_gemv<8>(a, (unsigned)grid, (size_t)smem, stream);
 }
+
+}  // namespace tmq

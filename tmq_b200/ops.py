@@ -744,9 +744,11 @@ def ternary_gemv_batched(x, wts, columns, scales=None, biases=None, out_dtype=to
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}      # TMQ_TYPE_*
 _A8_TYPES = {torch.int8: -1, **_TYPES}
+_GROUPED_TYPES = {torch.bfloat16: 1, torch.int8: -1}
+_I8_TYPES = {torch.int8: -1}
 I8_K_MAX = 131071        # int32 sums of 8-bit products are exact up to this length
 GROUPS_MAX = 512         # experts one grouped launch takes (TMQ_GROUPS_MAX)
-A8_TOKENS = 8            # rows the one-launch form (tmq_ternary_gemv_a8) takes
+A8_TOKENS = 8            # rows tmq_ternary_gemm_a8 quantises and multiplies in one launch
 _row_words = {}
 _status_address = {}
 
@@ -824,6 +826,14 @@ def _rows_out(name, out, M, N, dtype, device):
     return out, out.stride(0) if M > 1 else N, code
 
 
+def _code_scratch(code, M, K, device):
+    """Scratch for the codes and scales of floating-point activations (None for int8): stream-ordered caching allocator."""
+    if code < 0:
+        return None
+    n = lib().tmq_a8_workspace_bytes(code, M, K)
+    return torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device)
+
+
 def _check_packed(name, wt, N, K, fmt, device):
     words = _row_words.get((K, fmt))
     if words is None:
@@ -894,18 +904,16 @@ def ternary_gemm_a8(x, wt, columns, row_scale=None, scale=None, bias=None, out_d
     y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
-    rc = -6
-    if M <= A8_TOKENS:
-        x, ldx = _aligned_rows(x, M, K) if code < 0 else _unit_rows(x, M, K)
-        rc = _enqueue(lib().tmq_ternary_gemv_a8, dev.index, x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi,
-                      y.data_ptr(), y_code, M, N, K, ldy)
-    if rc == -6:               # more rows, or a matrix whose share per SM exceeds its shared memory
-        if code >= 0:
-            x, rs = quantize_rows(x)
-            p_rs = rs.data_ptr()
-        x, ldx = _aligned_rows(x, M, K)
-        rc = _enqueue(lib().tmq_ternary_gemm_a8, dev.index, x.data_ptr(), ldx, p_rs, wt.data_ptr(), p_sc, p_bi, y.data_ptr(),
-                      y_code, M, N, K, ldy)
+    x, ldx = _aligned_rows(x, M, K) if code < 0 else _unit_rows(x, M, K)
+    ws, nbytes, p_ws = None if M <= A8_TOKENS else _code_scratch(code, M, K, dev), 0, None
+    if ws is not None:
+        nbytes, p_ws = ws.numel(), ws.data_ptr()
+    rc = _enqueue(lib().tmq_ternary_gemm_a8, dev.index, x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi, y.data_ptr(),
+                  y_code, M, N, K, ldy, p_ws, nbytes)
+    if rc == -5:               # few rows, but a matrix whose share per SM exceeds its shared memory: not one launch
+        ws = _code_scratch(code, M, K, dev)
+        rc = _enqueue(lib().tmq_ternary_gemm_a8, dev.index, x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi,
+                      y.data_ptr(), y_code, M, N, K, ldy, ws.data_ptr(), ws.numel())
     if rc:
         check(rc, name)
     _launched(dev)
@@ -949,12 +957,10 @@ def gemm_i8(x, weight, row_scale=None, scale=None, bias=None, out_dtype=torch.bf
     y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
-    if code >= 0:
-        x, rs = quantize_rows(x)
-        p_rs = rs.data_ptr()
-    x, ldx = _aligned_rows(x, M, K)
-    rc = _enqueue(lib().tmq_gemm_i8, dev.index, x.data_ptr(), ldx, p_rs, weight.data_ptr(), ldw, p_sc, p_bi, y.data_ptr(),
-                  y_code, M, N, K, ldy)
+    x, ldx = _aligned_rows(x, M, K) if code < 0 else _unit_rows(x, M, K)
+    ws = _code_scratch(code, M, K, dev)
+    rc = _enqueue(lib().tmq_gemm_i8, dev.index, x.data_ptr(), code, ldx, p_rs, weight.data_ptr(), ldw, p_sc, p_bi, y.data_ptr(),
+                  y_code, M, N, K, ldy, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     if rc:
         check(rc, name)
     _launched(dev)
@@ -981,7 +987,7 @@ def ternary_gemm_grouped(x, wts, columns, offsets, row_scale=None, scales=None, 
     fresh result and left as they were in `out`.  Boundaries outside 0 .. M or out of order give empty or shortened groups.
     No gradient."""
     name = "ternary_gemm_grouped"
-    i8 = _rows_type(name, x, {torch.bfloat16: 1, torch.int8: -1}) < 0
+    i8 = _rows_type(name, x, _GROUPED_TYPES) < 0
     M, K = x.shape
     N = int(columns)
     dev = x.device
@@ -1017,7 +1023,7 @@ def gemm_i8_grouped(x, weights, offsets, row_scale=None, scales=None, biases=Non
     """ternary_gemm_grouped for 8-bit weights: weights int8 [experts, N, K] whose rows lie one behind the other and start at
     multiples of 16 bytes; x int8 [M, K] with row_scale fp32 [M].  Everything else as there."""
     name = "gemm_i8_grouped"
-    _rows_type(name, x, {torch.int8: -1})
+    _rows_type(name, x, _I8_TYPES)
     M, K = x.shape
     dev = x.device
     ldw = _check_i8_weights(name, weights, 3, dev)
