@@ -11,8 +11,11 @@ __all__ = ["CUDA_EXT_AVAILABLE", "NATIVE_EXT_AVAILABLE", "Conv2d", "ConvTranspos
            "quantize_model", "quantize_weights", "fwd_softstep", "bwd_softstep", "fwd_softstep_derivative",
            "bwd_softstep_derivative", "compactify_ternary", "expand_ternary", "compress_ternary", "decompress_ternary"]
 
+# reachable as tmq_b200.<name> without being part of the reference's star import
+_BEYOND = ("PackedExperts", "set_activation_bits")
+
 
 def __getattr__(name):
-    if name in __all__:
+    if name in __all__ or name in _BEYOND:
         return getattr(importlib.import_module(".tmq", __name__), name)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

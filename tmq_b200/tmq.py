@@ -471,6 +471,13 @@ class TMQLayer:
         w = self.weight.data
         return w.contiguous().view(-1, w.shape[-1])
 
+    def _channel_scale(self, n_out, device):
+        """post_scale as the fp32 [n_out] vector of the GEMM epilogue, or None for 1."""
+        if self.post_scale_imm == 1.0:
+            return None
+        return self._cached_layout(("post_scale", float(self.post_scale_imm)), lambda: torch.full(
+            (n_out,), float(self.post_scale_imm), dtype=torch.float32, device=device))
+
     def _compact_matmul(self, x2d, fuse=True):
         """[M, K] activations x packed weights -> [M, N] with post_scale and bias fused into the epilogue (fuse=False:
         the bare product).  fp32 in -> fp32 out (exact split), bf16 in -> bf16 out, int8 in -> int32 out (no scale /
@@ -540,6 +547,7 @@ class Linear(nn.Module, TMQLayer):
         self.post_scale_imm = 1.0 / (self._in_features * self._variance_estimate()) if post_scale else 1.0
         self.post_scale = nn.Parameter(torch.tensor(self.post_scale_imm), requires_grad=False)
         self.bn = None
+        self.activation_bits = None
 
     def __repr__(self):
         if len(self.original_shape) == 2:
@@ -578,13 +586,21 @@ class Linear(nn.Module, TMQLayer):
 
     @torch.no_grad()
     def compact_forward(self, x):
-        """Inference from the packed weights, any leading dimensions [tmq/tmq.py:662-688 handles one row only]."""
+        """Inference from the packed weights, any leading dimensions [tmq/tmq.py:662-688 handles one row only].  With
+        activation_bits = 8 (set_activation_bits) every row of floating-point activations is quantised to 8 bits with a scale
+        of its own; the result comes in the activations' type."""
         assert self.training == False, "Compact inference is not supported in training mode"
         assert self.weight.data.dtype == torch.int32, "Compact inference requires 32-bit integer words"
         _require_cuda(x, "compact_forward")
         self._update_scale()
         lead = x.shape[:-1]
-        out = self._compact_matmul(x.reshape(-1, x.shape[-1]))
+        x2d = x.reshape(-1, x.shape[-1])
+        if self.activation_bits == 8 and x.dtype != torch.int8:
+            n_out = self._gemm_columns()
+            out = ops.ternary_gemm_a8(x2d, self._prepacked_weights(ops.FMT_I8), n_out, scale=self._channel_scale(n_out, x.device),
+                                      bias=self.bias, out_dtype=x.dtype)
+        else:
+            out = self._compact_matmul(x2d)
         out = out.view(*lead, out.shape[-1])
         return self.bn(out) if self.bn is not None else out
 
@@ -609,6 +625,65 @@ class Linear(nn.Module, TMQLayer):
         super(Linear, self)._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys,
                                                   unexpected_keys, error_msgs)
         self._load_compact_metadata(state_dict, prefix, local_metadata)
+
+
+class PackedExperts(nn.Module):
+    """Packed Linear layers of one shape as the experts of one grouped product (inference only; no counterpart in the
+    reference, whose layers are called one by one).
+
+    layers: compact Linear layers (compressed_state_dict, load_compressed_state_dict) with equal shapes, on one GPU, without
+    an implicit batch norm.  Their weights are copied into one stack, their post_scale and bias into one table each; later
+    changes of the layers do not show.  activation_bits: None multiplies bf16 rows as they are (fp32 accumulation), 8
+    quantises each row (fp32, bf16 or fp16) to 8 bits with a scale of its own."""
+
+    def __init__(self, layers, activation_bits=None):
+        super().__init__()
+        layers = list(layers)
+        if activation_bits not in (None, 8):
+            raise ValueError("PackedExperts: activation_bits must be None or 8")
+        if not 1 <= len(layers) <= ops.GROUPS_MAX:
+            raise ValueError(f"PackedExperts: 1 .. {ops.GROUPS_MAX} layers")
+        for layer in layers:
+            if not isinstance(layer, Linear) or not layer.compact or layer.weight.data.dtype != torch.int32:
+                raise RuntimeError("PackedExperts: expected compact Linear layers with packed weights")
+            if tuple(layer.original_shape) != tuple(layers[0].original_shape) or layer.bn is not None:
+                raise RuntimeError("PackedExperts: the layers must have one shape and no implicit batch norm")
+            _require_cuda(layer.weight, "PackedExperts")
+            if layer.weight.device != layers[0].weight.device:
+                raise RuntimeError("PackedExperts: the layers must be on one GPU")
+            layer._update_scale()
+        self.out_features, self.in_features = (int(d) for d in layers[0].original_shape)
+        self.activation_bits = activation_bits
+        dev = layers[0].weight.device
+        fmt = ops.FMT_I8 if activation_bits == 8 else ops.FMT_BF16
+        with torch.no_grad():
+            weights = torch.stack([ops.prepack(layer._packed_matrix(), self.out_features, fmt) for layer in layers])
+            scales = biases = None
+            if any(layer.post_scale_imm != 1.0 for layer in layers):
+                scales = torch.tensor([float(layer.post_scale_imm) for layer in layers], device=dev)
+                scales = scales[:, None].expand(len(layers), self.out_features).contiguous()
+            if any(layer.bias is not None for layer in layers):
+                zero = torch.zeros(self.out_features, device=dev)
+                biases = torch.stack([zero if layer.bias is None else layer.bias.detach().float().to(dev) for layer in layers])
+        self.register_buffer("weights", weights, persistent=False)
+        self.register_buffer("scales", scales, persistent=False)
+        self.register_buffer("biases", biases, persistent=False)
+
+    def __repr__(self):
+        return "PackedExperts(%d x %d,%d) [tmq]" % (self.weights.shape[0], self.out_features, self.in_features)
+
+    @torch.no_grad()
+    def forward(self, x, offsets):
+        """x [M, in_features], rows sorted by expert; offsets: experts + 1 boundaries (int32 / int64, on the device, see
+        ops.ternary_gemm_grouped).  Returns [M, out_features] in x's type (bf16 without activation_bits)."""
+        _require_cuda(x, "PackedExperts")
+        if x.dim() != 2 or x.shape[1] != self.in_features:
+            raise RuntimeError("PackedExperts: expected [rows, in_features] activations")
+        row_scale, out_dtype = None, x.dtype
+        if self.activation_bits == 8:
+            x, row_scale = ops.quantize_rows(x)
+        return ops.ternary_gemm_grouped(x, self.weights, self.out_features, offsets, row_scale, self.scales, self.biases,
+                                        out_dtype=out_dtype)
 
 
 class Conv2d(nn.Module, TMQLayer):
@@ -893,6 +968,17 @@ def _tmq_layers(module, prefix=""):
             yield full, module, name, sub
         else:
             yield from _tmq_layers(sub, full)
+
+
+def set_activation_bits(module: nn.Module, bits):
+    """Precision of the activations in the compact (packed) inference of every TMQ Linear layer of `module`: 8 quantises each
+    row to 8 bits with a scale of its own (ops.ternary_gemm_a8), None multiplies the activations as they come.  Training and
+    uncompressed layers are not affected.  No counterpart in the reference."""
+    if bits not in (None, 8):
+        raise ValueError("set_activation_bits: bits must be None or 8")
+    for sub in module.modules():
+        if isinstance(sub, Linear):
+            sub.activation_bits = bits
 
 
 def quantize_weights(module: nn.Module):
