@@ -506,18 +506,23 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     const CUtensorMapDataType xt = C::I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const int xe = C::I8 ? 1 : 2;
     const int last = (int)(a.M % BN + 7) / 8 * 8;         // rows of a plain product's last tile
-    maps.height[0] = BN;
     maps.height[1] = a.groups > 1 ? BN / 2 : last ? last : BN;
     maps.height[2] = a.groups > 1 ? BN / 4 : maps.height[1];
+    maps.height[0] = a.groups == 1 && a.M < BN ? maps.height[1] : BN;        // a plain product without a full tile
     a.wide = a.K % C::BK == 0;
     const long long w_bytes = a.N * (C::DENSE ? p.ldw : prepack_row_words(a.K, C::I8 ? 1 : 0) * 4);
     // weights that do not stay in L2 between two row tiles (300 x 28672 x 8192 8-bit, 235 MB: 122 -> 82 us; up to 58 MB the two
     // orders are within 2 %)
     a.rows_first = a.groups == 1 && !a.offsets && w_bytes > (64ll << 20) && w_bytes > a.M * p.ldx * xe;
-    for (int i = 0; i < 3; i++)
+    for (int i = 0; i < 3; i++) {        // an encoding costs about half a microsecond: boxes of one height share it
+        if (i > 0 && maps.height[i] == maps.height[i - 1]) {
+            maps.x[i] = maps.x[i - 1];
+            continue;
+        }
         if (!make_map_blocks(maps.x + i, xt, xe, p.X, (uint64_t)a.K, (uint64_t)a.M, (uint64_t)p.ldx * xe, C::BK, maps.height[i],
                              C::KB, a.wide))
             return TMQ_ERR_LAUNCH;
+    }
     const uint64_t wrows = (uint64_t)a.groups * (uint64_t)a.N;
     const bool okw = C::DENSE
         ? make_map_blocks(&maps.w, xt, 1, p.W, (uint64_t)a.K, wrows, (uint64_t)p.ldw, C::BK, kTileC, C::KB, a.wide)

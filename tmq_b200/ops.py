@@ -464,6 +464,7 @@ class _StatusWatch:
     within about 2 * EVERY operator calls instead of never."""
 
     EVERY = 32
+    POLL = 8         # calls between two looks at a pending copy: an event query costs 1.5 us of host time
 
     def __init__(self, device):
         self.device = device
@@ -474,7 +475,8 @@ class _StatusWatch:
 
     def note_launch(self):
         # an event may not be queried while the stream is being captured: the capture would be lost
-        if self.pending and not torch.cuda.is_current_stream_capturing() and self.event.query():
+        if (self.pending and self.launches % self.POLL == 0 and not torch.cuda.is_current_stream_capturing()
+                and self.event.query()):
             self.pending = False
             code = int(self.host[0])
             if code != 0:
@@ -922,14 +924,16 @@ def ternary_gemm_a8(x, wt, columns, row_scale=None, scale=None, bias=None, out_d
 
 def _check_i8_weights(name, w, dims, device):
     """8-bit weights are read in place: the row stride of a stack [E, N, K] / matrix [N, K], or a refusal."""
-    if w.dtype != torch.int8 or w.device != device or w.dim() != dims or w.shape[-1] == 0 or w.shape[-2] == 0:
+    shape = w.shape
+    if w.dtype is not torch.int8 or w.device != device or len(shape) != dims or shape[-1] == 0 or shape[-2] == 0:
         raise RuntimeError(f"{name}: expected int8 weights {'[N, K]' if dims == 2 else '[experts, N, K]'} on the "
                            "activations' device")
-    N, K = w.shape[-2:]
-    ldw = w.stride(-2) if N > 1 else (K + 15) // 16 * 16
-    ok = (K == 1 or w.stride(-1) == 1) and ldw >= K and ldw % 16 == 0 and w.data_ptr() % 16 == 0
-    if dims == 3 and w.shape[0] > 1:
-        ok = ok and w.stride(0) == N * ldw
+    N, K = shape[-2:]
+    stride = w.stride()
+    ldw = stride[-2] if N > 1 else (K + 15) // 16 * 16
+    ok = (K == 1 or stride[-1] == 1) and ldw >= K and ldw % 16 == 0 and w.data_ptr() % 16 == 0
+    if dims == 3 and shape[0] > 1:
+        ok = ok and stride[0] == N * ldw
     if not ok:
         raise RuntimeError(f"{name}: the weights' rows must lie one behind the other, each starting at a multiple of 16 bytes "
                            "(pad the rows as quantize_rows does)")
