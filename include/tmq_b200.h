@@ -269,14 +269,14 @@ int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *scale, int64_
  *   row_scale fp32 [M] or NULL for 1.
  * x_type TMQ_TYPE_*: X holds floating point [M][ldx] (element-aligned) and is quantised first, exactly as tmq_quantize_rows
  *   does; row_scale NULL; workspace: tmq_a8_workspace_bytes(x_type, M, K) bytes of device scratch, 16-byte aligned
- *   (TMQ_ERR_SCRATCH without it, before anything is launched).  tmq_ternary_gemm_a8 needs none for M <= 8 where an SM's share
- *   of the matrix fits its shared memory (N <= 11840 and rows of a few thousand): quantisation and product are then one launch.
+ *   (TMQ_ERR_SCRATCH without it, before anything is launched).  tmq_ternary_gemm_a8 needs none for M <= 8 and
+ *   M K <= TMQ_A8_FUSED_ELEMS where an SM's share of the matrix fits its shared memory (N <= 11840 and rows of a few
+ *   thousand): quantisation and product are then one launch.
  * Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw], 16-byte aligned, ldw % 16 == 0.
  * Y [M][ldy], element-aligned.  *status: see "Status word" above.
- * tmq_ternary_gemm_a8 with M <= 8 fetches Wt ahead of the stream's previous kernel: the CONTRACT of tmq_ternary_gemv_bf16 holds
- * for Wt (not for scale, bias, row_scale, X).
  * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549, ternary_mvm_cuda, :563-603, and the post_scale / bias of
  * Linear.compact_forward, tmq/tmq.py:662-688 (fp32 activations on CUDA cores). */
+#define TMQ_A8_FUSED_ELEMS 16384
 size_t tmq_a8_workspace_bytes(int x_type, int64_t M, int64_t K);
 int tmq_ternary_gemm_a8(const void *X, int x_type, int64_t ldx, const float *row_scale, const uint32_t *Wt, const float *scale,
                         const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, void *workspace,

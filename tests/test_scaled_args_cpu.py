@@ -52,6 +52,7 @@ def test_product_arguments():
     assert i8(ldw=63) == -1 and i8(ldw=72) == -6
     assert a8(M=4, x_type=1, rs=P(4096)) == -1 and a8(M=4, X=P(4100)) == -2     # the one-launch form
     assert a8(M=4, x_type=1, N=12000, ldy=12000) == -5                     # too wide for it: scratch
+    assert a8(M=8, x_type=1, K=2064, ldx=2064) == -5                       # too many elements for it
 
 
 def test_scratch_size():

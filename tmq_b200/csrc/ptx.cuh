@@ -196,6 +196,11 @@ __device__ __forceinline__ void bulk_load(void *smem_dst, const void *gsrc, uint
                  : "memory");
 }
 
+// A run of global memory into L2 (16-byte aligned, size a multiple of 16 bytes)
+__device__ __forceinline__ void prefetch_l2(const void *gsrc, uint32_t bytes) {
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(gsrc)), "r"(bytes) : "memory");
+}
+
 // 256-bit global accesses (32-byte aligned): a lane moves a whole 32-byte sector with one request.  An epilogue whose
 // threads each own an output row otherwise writes every sector with two 16-byte requests from two instructions.
 struct u32x8 {

@@ -617,44 +617,47 @@ extern "C" size_t tmq_a8_workspace_bytes(int x_type, int64_t M, int64_t K) {
     return (size_t)(M * code_pitch(K) + 4 * M);
 }
 
-// Floating-point activations -> codes and scales in the workspace; p then describes the 8-bit product.
-static int quantize_operand(ScaledProblem &p, int x_type, void *workspace, size_t workspace_bytes, cudaStream_t st) {
+// Checks an 8-bit product's arguments and quantises floating-point activations into the workspace; p then describes the
+// product of the codes.  Nothing is launched for a call that is refused.
+static int prepare_a8(ScaledProblem &p, int x_type, bool dense, void *workspace, size_t workspace_bytes, cudaStream_t st) {
     ScaledArgs &a = p.a;
+    if (x_type < 0) return check_scaled(p, 1, dense);
     const int xe = x_type == TMQ_TYPE_F32 ? 4 : 2;
-    if (a.row_scale || p.ldx < a.K || a.K <= 0 || a.M < 0) return TMQ_ERR_ARG;
-    if (a.M == 0) return TMQ_OK;
-    if (!p.X) return TMQ_ERR_ARG;
-    if (!aligned(p.X, xe) || !aligned(workspace, 16)) return TMQ_ERR_ALIGN;
+    if (a.row_scale || a.K <= 0 || p.ldx < a.K || (a.M > 0 && !p.X)) return TMQ_ERR_ARG;
+    ScaledProblem q = p;
+    q.X = workspace;
+    q.ldx = code_pitch(a.K);
+    if (!workspace) q.X = reinterpret_cast<const void *>(uintptr_t(16));      // any aligned address: only the rest is looked at
+    int rc = check_scaled(q, 1, dense);
+    if (rc != TMQ_OK || a.M == 0) return rc;
+    if (!aligned(p.X, xe)) return TMQ_ERR_ALIGN;
     if (!workspace || workspace_bytes < tmq_a8_workspace_bytes(x_type, a.M, a.K)) return TMQ_ERR_SCRATCH;
     int8_t *codes = reinterpret_cast<int8_t *>(workspace);
-    float *scales = reinterpret_cast<float *>(codes + a.M * code_pitch(a.K));
-    const ScaledProblem before = p;
+    float *scales = reinterpret_cast<float *>(codes + a.M * q.ldx);
+    rc = tmq_quantize_rows(p.X, x_type, codes, scales, a.M, a.K, p.ldx, q.ldx, q.ldx, st);
     p.X = codes;
-    p.ldx = code_pitch(a.K);
+    p.ldx = q.ldx;
     a.row_scale = scales;
-    return tmq_quantize_rows(before.X, x_type, codes, scales, a.M, a.K, before.ldx, p.ldx, p.ldx, st);
+    return rc;
 }
 
 extern "C" int tmq_ternary_gemm_a8(const void *X, int x_type, int64_t ldx, const float *row_scale, const uint32_t *Wt,
                                    const float *scale, const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K,
                                    int64_t ldy, void *workspace, size_t workspace_bytes, int *status, void *stream) {
     if (x_type < -1 || x_type > TMQ_TYPE_F16) return TMQ_ERR_ARG;
-    if (M <= 8) {                        // one launch, unless an SM's share of the matrix is too large for it
-        const int rc = launch_token_product(X, x_type, ldx, row_scale, Wt, scale, bias, Y, y_type, M, N, K, ldy, status,
-                                            (cudaStream_t)stream);
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (M <= 8) {                        // one launch
+        const int rc = launch_token_product(X, x_type, ldx, row_scale, Wt, scale, bias, Y, y_type, M, N, K, ldy, status, st);
         if (rc != TMQ_ERR_UNSUPPORTED) return rc;
     }
     ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, status}};
-    ScaledProblem q = p;                 // arguments first: nothing is launched for a call that will be refused
-    if (x_type >= 0) {
-        q.X = workspace;
-        q.ldx = code_pitch(K);
-    }
-    int rc = check_scaled(q, 1, false);
-    if (x_type >= 0 && M > 0 && rc == TMQ_ERR_ARG && !workspace) rc = TMQ_ERR_SCRATCH;
+    int rc = prepare_a8(p, x_type, false, workspace, workspace_bytes, st);
     if (rc != TMQ_OK || M == 0) return rc;
-    if (x_type >= 0) rc = quantize_operand(p, x_type, workspace, workspace_bytes, (cudaStream_t)stream);
-    return rc != TMQ_OK ? rc : dispatch_scaled<W_TERNARY_I8>(p, (cudaStream_t)stream);
+    if (M <= 8 && x_type >= 0) {         // too many elements to quantise in every CTA, but few rows
+        rc = launch_token_product(p.X, -1, p.ldx, p.a.row_scale, Wt, scale, bias, Y, y_type, M, N, K, ldy, status, st);
+        if (rc != TMQ_ERR_UNSUPPORTED) return rc;
+    }
+    return dispatch_scaled<W_TERNARY_I8>(p, st);
 }
 
 extern "C" int tmq_gemm_i8(const void *X, int x_type, int64_t ldx, const float *row_scale, const int8_t *W, int64_t ldw,
@@ -662,16 +665,8 @@ extern "C" int tmq_gemm_i8(const void *X, int x_type, int64_t ldx, const float *
                            int64_t ldy, void *workspace, size_t workspace_bytes, int *status, void *stream) {
     if (x_type < -1 || x_type > TMQ_TYPE_F16) return TMQ_ERR_ARG;
     ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, status}};
-    ScaledProblem q = p;
-    if (x_type >= 0) {
-        q.X = workspace;
-        q.ldx = code_pitch(K);
-    }
-    int rc = check_scaled(q, 1, true);
-    if (x_type >= 0 && M > 0 && rc == TMQ_ERR_ARG && !workspace) rc = TMQ_ERR_SCRATCH;
-    if (rc != TMQ_OK || M == 0) return rc;
-    if (x_type >= 0) rc = quantize_operand(p, x_type, workspace, workspace_bytes, (cudaStream_t)stream);
-    return rc != TMQ_OK ? rc : dispatch_scaled<W_DENSE_I8>(p, (cudaStream_t)stream);
+    const int rc = prepare_a8(p, x_type, true, workspace, workspace_bytes, (cudaStream_t)stream);
+    return rc != TMQ_OK || M == 0 ? rc : dispatch_scaled<W_DENSE_I8>(p, (cudaStream_t)stream);
 }
 
 extern "C" int tmq_ternary_gemm_grouped_bf16(const void *X, int64_t ldx, const uint32_t *Wt, const float *scale,

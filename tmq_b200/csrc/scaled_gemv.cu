@@ -3,11 +3,13 @@
 //
 // The decode step of a language model is a chain of such products, each a few microseconds long, so what counts is the
 // number of launches and what a launch does before its first multiplication.  A CTA owns up to five groups of 16 channels
-// and bulk-copies their packed rows (one contiguous run) into shared memory BEFORE it waits for its predecessor in the
-// stream; after the wait every CTA reads the few rows of X (they sit in L2), finds their maxima and quantises them into
-// shared memory for itself - 148 times the same 8 KB cost less than a second launch and its hand-over - and multiplies:
-// byte dot products for one or two rows, warp-level int8 MMA (the rows as its eight columns) for more.  Sums are exact, so
-// the order of the warps' slices does not show.
+// and asks for their packed rows (one contiguous run) to be brought into L2 BEFORE it waits for its predecessor in the stream -
+// only that: L2 is where a predecessor's writes arrive, so weights it has just written are seen all the same - and copies them
+// into shared memory after the wait, while every CTA reads the few rows of X, finds their maxima and quantises them into
+// shared memory for itself: up to TMQ_A8_FUSED_ELEMS elements, 148 times the same 8 KB cost less than a second launch and its hand-over.
+// Then it multiplies with warp-level int8 MMAs, the rows as their eight columns (byte dot products for one row measured 5.9
+// against 6.2 us on 11008 x 4096, 3.2 against 2.8 us on 1024 x 2048).  Sums are exact, so the order of the warps' slices does
+// not show.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,16 +38,10 @@ struct ScaledGemvArgs {
     int *status;
 };
 
-__device__ __forceinline__ void store_result(void *Y, int y_type, long long i, float f) {
-    if (y_type == TMQ_TYPE_F32) reinterpret_cast<float *>(Y)[i] = f;
-    else if (y_type == TMQ_TYPE_BF16) reinterpret_cast<__nv_bfloat16 *>(Y)[i] = __float2bfloat16_rn(f);
-    else reinterpret_cast<__half *>(Y)[i] = __float2half_rn(f);
-}
-
 // Rows of X -> codes in shared memory (zero from K to the row pitch) and their scales.  16 / MP warps share a row.
 template <typename T, int MP>
 __device__ __forceinline__ void quantize_to_smem(const ScaledGemvArgs &a, uint8_t *xq, float *row_scale, uint32_t *red) {
-    constexpr int WPR = kSgWarps / MP, V = QuantType<T>::V, STEP = WPR * 32 * V, CH = MP == 8 ? 8 : 4;
+    constexpr int WPR = kSgWarps / MP, V = QuantType<T>::V, STEP = WPR * 32 * V, CH = 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int m = warp / WPR, t = (warp % WPR) * 32 + lane;
     const bool live = m < a.M;
@@ -53,18 +49,18 @@ __device__ __forceinline__ void quantize_to_smem(const ScaledGemvArgs &a, uint8_
     const int K = live ? (int)a.K : 0;
     QuantVec<T> held[CH];
     uint32_t peak = 0;
-    auto load = [&](QuantVec<T> &v, int k) {
-        if (a.vload) v.template load<true>(x, k, K);
-        else v.template load<false>(x, k, K);
+    // CH vectors at a time, all of them on their way before the first is looked at
+    auto load = [&](int base) {
+#pragma unroll
+        for (int c = 0; c < CH; c++) {
+            if (a.vload) held[c].template load<true>(x, base + c * STEP + t * V, K);
+            else held[c].template load<false>(x, base + c * STEP + t * V, K);
+        }
     };
+    for (int base = 0; base == 0 || base < K; base += CH * STEP) {
+        load(base);
 #pragma unroll
-    for (int c = 0; c < CH; c++) load(held[c], c * STEP + t * V);
-#pragma unroll
-    for (int c = 0; c < CH; c++) held[c].peak(peak);
-    for (int k = CH * STEP + t * V; k < K; k += STEP) {
-        QuantVec<T> v;
-        load(v, k);
-        v.peak(peak);
+        for (int c = 0; c < CH; c++) held[c].peak(peak);
     }
     peak = __reduce_max_sync(0xffffffffu, QuantType<T>::fold(peak));
     if (lane == 0) red[warp] = peak;
@@ -75,19 +71,18 @@ __device__ __forceinline__ void quantize_to_smem(const ScaledGemvArgs &a, uint8_
     const RowQuant<T> rq(peak);
     if (t == 0) row_scale[m] = rq.scale;
     uint8_t *q = xq + m * a.x_pitch;
-    auto put = [&](const QuantVec<T> &v, int k) {
-        if (k >= a.x_pitch) return;
-        uint32_t c[V / 4];
-        v.codes(rq, c);
-        if (V == 8) *reinterpret_cast<uint2 *>(q + k) = make_uint2(c[0], c[V / 4 - 1]);
-        else *reinterpret_cast<uint32_t *>(q + k) = c[0];
-    };
+    for (int base = 0; base < a.x_pitch; base += CH * STEP) {
+        if (K > CH * STEP) load(base);                   // a row that fits the registers is still in them
 #pragma unroll
-    for (int c = 0; c < CH; c++) put(held[c], c * STEP + t * V);
-    for (int k = CH * STEP + t * V; k < a.x_pitch; k += STEP) {
-        QuantVec<T> v;
-        load(v, k);
-        put(v, k);
+        for (int c = 0; c < CH; c++) {
+            const int k = base + c * STEP + t * V;
+            if (k < a.x_pitch) {
+                uint32_t d[V / 4];
+                held[c].codes(rq, d);
+                if (V == 8) *reinterpret_cast<uint2 *>(q + k) = make_uint2(d[0], d[V / 4 - 1]);
+                else *reinterpret_cast<uint32_t *>(q + k) = d[0];
+            }
+        }
     }
 }
 
@@ -110,20 +105,11 @@ __device__ __forceinline__ void copy_codes(const ScaledGemvArgs &a, uint8_t *xq,
     if (threadIdx.x < a.M) row_scale[threadIdx.x] = a.row_scale ? a.row_scale[threadIdx.x] : 1.0f;
 }
 
-__device__ __forceinline__ uint4 lds_16(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-
 // MP: rows rounded up to a power of two.  Lane (g, t) of a warp owns channels g and g + 8 of every group and 64 k of each
 // 256-wide slice; warps take the slices round-robin.  Words a lane reads past the valid part of its row (row padding, the
 // next row, the slack behind the last) meet codes that are zero, and any bits decode to finite numbers.
 template <int MP>
-__global__ void __launch_bounds__(kSgWarps * 32, MP <= 2 ? 2 : 1) scaled_gemv_kernel(const ScaledGemvArgs a) {
-    constexpr bool DOT = MP <= 2;
-    constexpr int RL = 2 * kSgGroups;                    // channels per lane
-    constexpr int MC = DOT ? MP : 8;                     // accumulator columns
+__global__ void __launch_bounds__(kSgWarps * 32, 1) scaled_gemv_kernel(const ScaledGemvArgs a) {
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ __align__(8) uint64_t bar;
     __shared__ float row_scale[8];
@@ -134,16 +120,19 @@ __global__ void __launch_bounds__(kSgWarps * 32, MP <= 2 ? 2 : 1) scaled_gemv_ke
     const int g = lane >> 2, t = lane & 3;
     const int group0 = (int)((blockIdx.x * (unsigned)a.ngroups) / gridDim.x);
     const int G = (int)(((blockIdx.x + 1) * (unsigned)a.ngroups) / gridDim.x) - group0;
+    // this CTA's packed rows, one contiguous run of whole 64-byte blocks
+    const uint32_t *rows = a.Wt + (long long)group0 * 16 * a.KS;
+    const uint32_t bytes = (uint32_t)((a.N - (long long)group0 * 16 < G * 16 ? a.N - (long long)group0 * 16 : G * 16) * a.KS * 4);
     if (threadIdx.x == 0) {
-        long long rows = a.N - (long long)group0 * 16;
-        if (rows > G * 16) rows = G * 16;
-        const uint32_t bytes = (uint32_t)(rows * a.KS * 4);
+        ptx::prefetch_l2(rows, bytes);
         ptx::mbar_init(&bar, 1);
         ptx::fence_mbar_init();
-        ptx::mbar_arrive_expect_tx(&bar, bytes);
-        ptx::bulk_load(smem, a.Wt + (long long)group0 * 16 * a.KS, bytes, &bar);
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (threadIdx.x == 0) {
+        ptx::mbar_arrive_expect_tx(&bar, bytes);
+        ptx::bulk_load(smem, rows, bytes, &bar);
+    }
     const bool healthy = *reinterpret_cast<volatile int *>(a.status) == 0;
     if (a.x_type < 0) copy_codes(a, xq, row_scale);
     else if (a.x_type == TMQ_TYPE_F32) quantize_to_smem<float, MP>(a, xq, row_scale, red16);
@@ -154,103 +143,57 @@ __global__ void __launch_bounds__(kSgWarps * 32, MP <= 2 ? 2 : 1) scaled_gemv_ke
     const bool ok = __syncthreads_and(ptx::mbar_wait_own(&bar, 0, a.status) && healthy);
     if (!ok) return;
 
-    int acc[RL][DOT ? MP : 1];                           // DOT: channel i * 8 + g, row m
-    int frag[kSgGroups][4];                              // MMA accumulators
-#pragma unroll
-    for (int i = 0; i < RL; i++)
-#pragma unroll
-        for (int m = 0; m < (DOT ? MP : 1); m++) acc[i][m] = 0;
+    int acc[kSgGroups][4];
 #pragma unroll
     for (int i = 0; i < kSgGroups; i++)
 #pragma unroll
-        for (int m = 0; m < 4; m++) frag[i][m] = 0;
+        for (int j = 0; j < 4; j++) acc[i][j] = 0;
 
     const int nslices = (int)((a.K + 255) / 256);
     const uint32_t row8 = (uint32_t)a.KS * 32u;
     const uint32_t wbase = ptx::smem_u32(smem) + (uint32_t)g * ((uint32_t)a.KS * 4u) + 16u * t;
-    const uint32_t xbase = ptx::smem_u32(xq) + 64u * t;
+    const uint32_t xbase = ptx::smem_u32(xq) + (uint32_t)(g * a.x_pitch) + 64u * t;
     for (int slice = warp; slice < nslices; slice += kSgWarps) {
-        uint32_t xr[DOT ? MP : 1][16];
+        uint32_t x[16];                                  // row g's 64 codes
 #pragma unroll
-        for (int m = 0; m < (DOT ? MP : 1); m++) {
-            const int row = DOT ? m : g;
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (row < a.M) v = lds_16(xbase + (uint32_t)(row * a.x_pitch + slice * 256 + 16 * q));
-                xr[m][4 * q] = v.x; xr[m][4 * q + 1] = v.y; xr[m][4 * q + 2] = v.z; xr[m][4 * q + 3] = v.w;
-            }
+        for (int q = 0; q < 4; q++) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (g < a.M) v = ptx::lds_v4(xbase + (uint32_t)(slice * 256 + 16 * q));
+            x[4 * q] = v.x; x[4 * q + 1] = v.y; x[4 * q + 2] = v.z; x[4 * q + 3] = v.w;
         }
         const uint32_t w0 = wbase + 64u * (uint32_t)slice;
-        if (DOT) {
 #pragma unroll
-            for (int i = 0; i < RL; i++) {
-                if (i < 2 * G) {
-                    const uint4 p = lds_16(w0 + (uint32_t)i * row8);
-                    const uint32_t words[4] = {p.x, p.y, p.z, p.w};
+        for (int i = 0; i < kSgGroups; i++) {
+            if (i < G) {
+                const uint4 p = ptx::lds_v4(w0 + (uint32_t)i * (2u * row8)), r = ptx::lds_v4(w0 + (uint32_t)i * (2u * row8) + row8);
+                const uint32_t lo[4] = {p.x, p.y, p.z, p.w}, hi[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        uint32_t d[4];
-                        decode_word_i8_ptx(words[w], d);
+                for (int w = 0; w < 4; w++) {
+                    uint32_t dl[4], dh[4];
+                    decode_word_i8_ptx(lo[w], dl);
+                    decode_word_i8_ptx(hi[w], dh);
 #pragma unroll
-                        for (int m = 0; m < (DOT ? MP : 1); m++)
-#pragma unroll
-                            for (int q = 0; q < 4; q++) acc[i][m] = __dp4a((int)d[q], (int)xr[m][4 * w + q], acc[i][m]);
-                    }
-                }
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < kSgGroups; i++) {
-                if (i < G) {
-                    const uint4 p = lds_16(w0 + (uint32_t)i * (2u * row8)), r = lds_16(w0 + (uint32_t)i * (2u * row8) + row8);
-                    const uint32_t lo[4] = {p.x, p.y, p.z, p.w}, hi[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        uint32_t dl[4], dh[4];
-                        decode_word_i8_ptx(lo[w], dl);
-                        decode_word_i8_ptx(hi[w], dh);
-#pragma unroll
-                        for (int h = 0; h < 2; h++)
-                            asm volatile(
-                                "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                                : "+r"(frag[i][0]), "+r"(frag[i][1]), "+r"(frag[i][2]), "+r"(frag[i][3])
-                                : "r"(dl[2 * h]), "r"(dh[2 * h]), "r"(dl[2 * h + 1]), "r"(dh[2 * h + 1]),
-                                  "r"(xr[0][4 * w + 2 * h]), "r"(xr[0][4 * w + 2 * h + 1]));
-                    }
+                    for (int h = 0; h < 2; h++)
+                        asm volatile(
+                            "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                            : "+r"(acc[i][0]), "+r"(acc[i][1]), "+r"(acc[i][2]), "+r"(acc[i][3])
+                            : "r"(dl[2 * h]), "r"(dh[2 * h]), "r"(dl[2 * h + 1]), "r"(dh[2 * h + 1]), "r"(x[4 * w + 2 * h]),
+                              "r"(x[4 * w + 2 * h + 1]));
                 }
             }
         }
     }
-    if (DOT) {
-#pragma unroll
-        for (int i = 0; i < RL; i++)
-#pragma unroll
-            for (int m = 0; m < (DOT ? MP : 1); m++) {
-                acc[i][m] += __shfl_xor_sync(0xffffffffu, acc[i][m], 1);
-                acc[i][m] += __shfl_xor_sync(0xffffffffu, acc[i][m], 2);
-            }
-    }
     __syncthreads();                                     // the packed rows are read: their area takes the warps' sums
-    int *red = reinterpret_cast<int *>(smem);            // [warp][channel of the CTA][MC]
-    if (DOT) {
-        if (t == 0)
+    int *red = reinterpret_cast<int *>(smem);            // [warp][channel of the CTA][8 rows]
 #pragma unroll
-            for (int i = 0; i < RL; i++)
-                if (i < 2 * G)
-#pragma unroll
-                    for (int m = 0; m < (DOT ? MP : 1); m++) red[(warp * (RL * 8) + i * 8 + g) * MC + m] = acc[i][m];
-    } else {
-#pragma unroll
-        for (int i = 0; i < kSgGroups; i++)
-            if (i < G) {
-                int *r = red + (warp * (RL * 8) + i * 16) * MC;
-                r[g * MC + 2 * t] = frag[i][0];
-                r[g * MC + 2 * t + 1] = frag[i][1];
-                r[(g + 8) * MC + 2 * t] = frag[i][2];
-                r[(g + 8) * MC + 2 * t + 1] = frag[i][3];
-            }
-    }
+    for (int i = 0; i < kSgGroups; i++)
+        if (i < G) {
+            int *r = red + (warp * (kSgGroups * 16) + i * 16) * 8 + 2 * t;
+            r[g * 8] = acc[i][0];
+            r[g * 8 + 1] = acc[i][1];
+            r[(g + 8) * 8] = acc[i][2];
+            r[(g + 8) * 8 + 1] = acc[i][3];
+        }
     __syncthreads();
     const int warps = nslices < kSgWarps ? nslices : kSgWarps;
     for (int o = threadIdx.x; o < G * 16 * (int)a.M; o += kSgWarps * 32) {
@@ -258,9 +201,9 @@ __global__ void __launch_bounds__(kSgWarps * 32, MP <= 2 ? 2 : 1) scaled_gemv_ke
         const long long n = (long long)group0 * 16 + c;
         if (n < a.N) {
             int s = 0;
-            for (int w = 0; w < warps; w++) s += red[(w * (RL * 8) + c) * MC + m];
+            for (int w = 0; w < warps; w++) s += red[(w * (kSgGroups * 16) + c) * 8 + m];
             const float f = fmaf(__fmul_rn(__int2float_rn(s), row_scale[m]), a.scale ? a.scale[n] : 1.0f, a.bias ? a.bias[n] : 0.0f);
-            store_result(a.Y, a.y_type, m * a.ldy + n, f);
+            store_one(a.Y, a.y_type, m * a.ldy + n, f);
         }
     }
 }
@@ -286,14 +229,13 @@ int launch_token_product(const void *X, int x_type, int64_t ldx, const float *ro
         !aligned(scale, 4) || !aligned(bias, 4) || !aligned(Y, y_type == TMQ_TYPE_F32 ? 4 : 2))
         return TMQ_ERR_ALIGN;
     const long long ngroups = (N + 15) / 16, grid = ngroups < kNumSMs ? ngroups : kNumSMs, G = (ngroups + grid - 1) / grid;
-    if (M > 8 || K > 131071 || G > kSgGroups) return TMQ_ERR_UNSUPPORTED;
-    const int mc = M <= 2 ? (int)M : 8;
+    if (M > 8 || K > 131071 || G > kSgGroups || (x_type >= 0 && M * K > TMQ_A8_FUSED_ELEMS)) return TMQ_ERR_UNSUPPORTED;
     ScaledGemvArgs a = {X, row_scale, Wt, scale, bias, Y, M, N, K, prepack_row_words(K, 1), ldx, ldy, x_type, y_type, vload};
     a.ngroups = (int)ngroups;
     a.status = status;
     a.x_pitch = (int)((K + 255) / 256 * 256);
     // packed rows (64 bytes of slack: a lane reads up to 48 behind the last row), later the warps' sums; then the codes
-    long long rows = G * 16 * a.KS * 4 + 64, red = (long long)kSgWarps * 2 * kSgGroups * 8 * mc * 4;
+    long long rows = G * 16 * a.KS * 4 + 64, red = (long long)kSgWarps * kSgGroups * 16 * 8 * 4;
     if (rows < red) rows = red;
     a.x_offset = (int)((rows + 127) / 128 * 128);
     const long long smem = a.x_offset + M * a.x_pitch;

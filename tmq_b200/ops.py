@@ -750,7 +750,8 @@ _GROUPED_TYPES = {torch.bfloat16: 1, torch.int8: -1}
 _I8_TYPES = {torch.int8: -1}
 I8_K_MAX = 131071        # int32 sums of 8-bit products are exact up to this length
 GROUPS_MAX = 512         # experts one grouped launch takes (TMQ_GROUPS_MAX)
-A8_TOKENS = 8            # rows tmq_ternary_gemm_a8 quantises and multiplies in one launch
+A8_TOKENS = 8            # rows, and elements, tmq_ternary_gemm_a8 quantises and multiplies in one launch
+A8_FUSED_ELEMS = 16384
 _row_words = {}
 _status_address = {}
 
@@ -885,7 +886,7 @@ def ternary_gemm_a8(x, wt, columns, row_scale=None, scale=None, bias=None, out_d
     """Y[m][n] = row_scale[m] * scale[n] * sum_k x[m][k] T[n][k] + bias[n] with 8-bit activations and packed ternary
     weights; the sums are exact, the scaling is fp32, the result bf16, fp16 or fp32 [M, columns].
     x: CUDA int8 [M, K] (any row stride; row_scale fp32 [M] or None for 1), or fp32 / bf16 / fp16 [M, K], which is quantised
-    here exactly as quantize_rows does (inside the product's launch for up to A8_TOKENS rows).  wt: prepack(..., FMT_I8).
+    here exactly as quantize_rows does (inside the product's launch for a few rows).  wt: prepack(..., FMT_I8).
     scale, bias: fp32 [columns] or None.  out: optional [M, columns] tensor of the output dtype whose rows may be strided.
     No gradient."""
     name = "ternary_gemm_a8"
@@ -907,7 +908,9 @@ def ternary_gemm_a8(x, wt, columns, row_scale=None, scale=None, bias=None, out_d
     if M == 0:
         return y
     x, ldx = _aligned_rows(x, M, K) if code < 0 else _unit_rows(x, M, K)
-    ws, nbytes, p_ws = None if M <= A8_TOKENS else _code_scratch(code, M, K, dev), 0, None
+    ws, nbytes, p_ws = None, 0, None
+    if M > A8_TOKENS or M * K > A8_FUSED_ELEMS:
+        ws = _code_scratch(code, M, K, dev)
     if ws is not None:
         nbytes, p_ws = ws.numel(), ws.data_ptr()
     rc = _enqueue(lib().tmq_ternary_gemm_a8, dev.index, x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi, y.data_ptr(),
