@@ -78,6 +78,18 @@ struct RowQuant {
     }
 };
 
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
 template <typename T>
 struct QuantVec {
     static constexpr int V = QuantType<T>::V;
@@ -110,12 +122,17 @@ struct QuantVec {
         const float magic = 12582912.0f;                 // 1.5 * 2^23
         float far = 0.0f;                                // largest remainder of the roundings
         uint32_t b[V];
+        const uint64_t inv2 = pack2(rq.inv, rq.inv), magic2 = pack2(magic, magic), minus2 = pack2(-1.0f, -1.0f);
 #pragma unroll
-        for (int i = 0; i < V; i++) {
-            const float x = QuantType<T>::get(w, i);
-            const float r = fmaf(x, rq.inv, magic);
-            far = fmaxf(far, fabsf(fmaf(x, rq.inv, magic - r)));
-            b[i] = __float_as_uint(r);
+        for (int i = 0; i < V; i += 2) {                 // two elements per instruction
+            const uint64_t x = pack2(QuantType<T>::get(w, i), QuantType<T>::get(w, i + 1));
+            const uint64_t r = fma2(x, inv2, magic2);
+            const uint64_t d = fma2(x, inv2, fma2(r, minus2, magic2));
+            float lo, hi;
+            unpack2(d, lo, hi);
+            far = fmaxf(far, fmaxf(fabsf(lo), fabsf(hi)));
+            b[i] = (uint32_t)r;
+            b[i + 1] = (uint32_t)(r >> 32);
         }
         // the quotient is off by at most 127 * 2^-24, the remainder by as much again: 2e-5 covers both
         if (far > 0.49998f || rq.tiny) {
