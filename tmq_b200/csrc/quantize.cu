@@ -27,8 +27,8 @@ template <typename T, bool VLOAD, int TPR, int CH>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
     constexpr int ROWS = 256 / TPR, V = QuantType<T>::V;
     __shared__ uint32_t red[8];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int t = threadIdx.x % TPR;
     const long long m = (long long)blockIdx.x * ROWS + threadIdx.x / TPR;
     const bool live = m < a.M;

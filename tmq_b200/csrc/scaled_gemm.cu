@@ -175,7 +175,6 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
     const int nkb = (int)((a.K + C::BK - 1) / C::BK);
     const int tiles_n = (int)((a.N + kTileC - 1) / kTileC);
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::NB; s++) {
             ptx::mbar_init(full + s, 1);
@@ -208,11 +207,13 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
     __syncthreads();
     ptx::tc_fence_after_sync();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t *>(tmem_slot);
-    const bool healthy = (*reinterpret_cast<volatile int *>(a.status) == 0);
+    // The next launch may set itself up beside this one from here on: this CTA holds its tensor memory, so it cannot be kept
+    // from it by a successor that waits for this grid.
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer (whole warp walks, one lane issues)
-        if (healthy) {
+        {
             int s = 0, round = 0;
             uint32_t ph = 1;
             bool ok = true;
@@ -250,7 +251,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (whole warp walks, one lane issues)
-        if (healthy) {
+        {
             int sa = 0, sb = 0, ti = 0;
             uint32_t pa = 0, pb = 0;
             bool ok = true, landed = false;
@@ -314,7 +315,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         }
     } else if (warp == 2) {
         // ---------------------------------------------------------------- TMA producer of the packed words
-        if (!C::DENSE && healthy) {
+        if (!C::DENSE) {
             int s = 0, round = 0;
             uint32_t ph = 1;
             bool ok = true;
@@ -346,7 +347,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         const uint32_t a_lane = tmem_base + ((uint32_t)(quarter * 32) << 16) + C::A_BASE;
         const uint32_t ready0 = ptx::smem_u32(ready), taken0 = ptx::smem_u32(taken), raw_full0 = ptx::smem_u32(raw_full),
                        raw_empty0 = ptx::smem_u32(raw_empty);
-        bool ok = healthy;
+        bool ok = true;
         int s = 0, rs = 0, turn = 0;
         uint32_t ph = 1, rph = 0;                        // parities: slot taken by the MMAs, box landed
         for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next()) {
@@ -433,7 +434,10 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         constexpr int kStep = 8 * C::EPI;                 // rows the epilogue warps of a quarter take per round
         float *rs = reinterpret_cast<float *>(smem + C::RS_OFF) + (warp - C::FIRST_EPI) * 32;
         const bool pairs = a.y_type != TMQ_TYPE_F32 && (a.ldy & 1) == 0 && (reinterpret_cast<uintptr_t>(a.Y) & 3) == 0;
-        bool ok = healthy;
+        // A set status word means that results are not to be touched; it is read here, where its latency is hidden, and not
+        // before the first copies (700 cycles of every launch).
+        const bool healthy = (*reinterpret_cast<volatile int *>(a.status) == 0);
+        bool ok = true;
         int ti = 0;
         for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next(), ti++) {
             const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
@@ -473,7 +477,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                     ptx::tmem_ld_x16(lane_addr + (uint32_t)c + 16, reinterpret_cast<uint32_t(&)[16]>(v[16]));
                     ptx::tmem_ld_wait();
                     if (left <= kStep) release();
-                    finish_rows<C::I8, 32>(v, rs, sc, bi, a, pairs, q.row0 + c, n, left, lane);
+                    if (healthy) finish_rows<C::I8, 32>(v, rs, sc, bi, a, pairs, q.row0 + c, n, left, lane);
                 } else {
 #pragma unroll 1
                     for (int j = 0; j < left; j += 8) {
@@ -481,7 +485,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                         ptx::tmem_ld_x8(lane_addr + (uint32_t)(c + j), v);
                         ptx::tmem_ld_wait();
                         if (left - j <= 8) release();
-                        finish_rows<C::I8, 8>(v, rs + j, sc, bi, a, pairs, q.row0 + c + j, n, left - j, lane);
+                        if (healthy) finish_rows<C::I8, 8>(v, rs + j, sc, bi, a, pairs, q.row0 + c + j, n, left - j, lane);
                     }
                 }
             }

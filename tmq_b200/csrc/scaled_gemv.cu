@@ -115,7 +115,6 @@ __global__ void __launch_bounds__(kSgWarps * 32, 1) scaled_gemv_kernel(const Sca
     __shared__ float row_scale[8];
     __shared__ uint32_t red16[kSgWarps];
     uint8_t *xq = smem + a.x_offset;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int group0 = (int)((blockIdx.x * (unsigned)a.ngroups) / gridDim.x);
@@ -129,6 +128,7 @@ __global__ void __launch_bounds__(kSgWarps * 32, 1) scaled_gemv_kernel(const Sca
         ptx::fence_mbar_init();
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         ptx::mbar_arrive_expect_tx(&bar, bytes);
         ptx::bulk_load(smem, rows, bytes, &bar);
