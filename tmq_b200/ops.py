@@ -464,7 +464,7 @@ class _StatusWatch:
     within about 2 * EVERY operator calls instead of never."""
 
     EVERY = 32
-    POLL = 8         # calls between two looks at a pending copy: an event query costs 1.5 us of host time
+    POLL = 8         # launches between two looks: an event query alone costs 1.5 us of host time
 
     def __init__(self, device):
         self.device = device
@@ -474,15 +474,15 @@ class _StatusWatch:
         self.launches = 0
 
     def note_launch(self):
-        # an event may not be queried while the stream is being captured: the capture would be lost
-        if (self.pending and self.launches % self.POLL == 0 and not torch.cuda.is_current_stream_capturing()
-                and self.event.query()):
+        self.launches += 1
+        if self.launches % self.POLL != 1 or torch.cuda.is_current_stream_capturing():
+            return                                # (a query would invalidate a capture, a copy would become part of it)
+        if self.pending and self.event.query():
             self.pending = False
             code = int(self.host[0])
             if code != 0:
                 _raise_status(self.device, code)
-        self.launches += 1
-        if not self.pending and self.launches % self.EVERY == 1 and not torch.cuda.is_current_stream_capturing():
+        if not self.pending and self.launches % self.EVERY == 1:
             self.host.copy_(gemm_status_word(self.device), non_blocking=True)
             self.event.record()
             self.pending = True
@@ -795,9 +795,11 @@ def _rows_type(name, x, types):
 
 def _unit_rows(x, M, K):
     """(tensor, row stride) with unit column stride and rows that do not overlap."""
-    if (x.stride(1) != 1 and K > 1) or (M > 1 and x.stride(0) < K):
+    if M == 1:
+        return x if K == 1 or x.stride(1) == 1 else x.contiguous(), (K + 15) // 16 * 16
+    if (x.stride(1) != 1 and K > 1) or x.stride(0) < K:
         x = x.contiguous()
-    return x, x.stride(0) if M > 1 else (K + 15) // 16 * 16
+    return x, x.stride(0)
 
 
 def _aligned_rows(x, M, K):
