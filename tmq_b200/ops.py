@@ -755,61 +755,77 @@ A8_FUSED_ELEMS = 16384
 _row_words = {}
 _status_address = {}
 
-# The calls below are a few microseconds long for single tokens: their host side avoids everything that costs as much
-# (torch.empty with a shape tuple, stream objects, device contexts for the device that is current anyway).
+# The calls below are a few microseconds long for single tokens, and their host side is kept to as little: one pass over the
+# arguments, torch.empty_strided (torch.empty with a shape tuple costs a microsecond more), raw streams, no device context for
+# the device that is current anyway.
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _enqueue(fn, index, *args):
-    """fn(*args, status word, stream) on the current stream of device `index`, which is made the current device for the call;
-    returns the status."""
-    word = _status_address.get(index)
-    if word is None:
-        word = _status_address[index] = gemm_status_word(torch.device("cuda", index)).data_ptr()
-    if torch.cuda.current_device() == index:
-        return fn(*args, word, torch._C._cuda_getCurrentRawStream(index))
+def _status_word_address(index):
+    word = _status_address[index] = gemm_status_word(torch.device("cuda", index)).data_ptr()
+    return word
+
+
+def _enqueue(fn, index, args):
+    """fn(*args) with `index` as the current device."""
+    if _current_device() == index:
+        return fn(*args)
     with torch.cuda.device(index):
-        return fn(*args, word, torch._C._cuda_getCurrentRawStream(index))
+        return fn(*args)
 
 
 def _vector(name, what, t, shape, device):
-    """(tensor, address) of an optional fp32 vector; the tensor is to be kept until the launch."""
-    if t is None:
-        return None, None
+    """An fp32 vector as the kernels read it; to be kept until the launch."""
     if t.shape != shape:
         raise RuntimeError(f"{name}: {what} must have shape {list(shape)}")
     if t.dtype is not torch.float32 or t.device != device or not t.is_contiguous():
         t = t.detach().to(device=device, dtype=torch.float32).contiguous()
-    return t, t.data_ptr()
+    return t
 
 
-def _rows_type(name, x, types):
-    """TMQ_TYPE of a 2-D CUDA tensor (-1: int8) or a refusal."""
-    code = types.get(x.dtype) if isinstance(x, torch.Tensor) else None
-    if code is None or not x.is_cuda or x.dim() != 2:
+def _refuse_rows(name, x, types):
+    if not isinstance(x, torch.Tensor) or x.dtype not in types or not x.is_cuda or x.dim() != 2:
         raise RuntimeError(f"{name}: expected a 2-D CUDA activation tensor of type "
                            + " / ".join(str(d).replace("torch.", "") for d in types))
     if x.shape[1] == 0:
         raise RuntimeError(f"{name}: rows without elements")
-    return code
+    raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
+
+
+def _rows_in(name, x, types, k_max=I8_K_MAX):
+    """(TMQ_TYPE, rows, columns, device) of a 2-D CUDA tensor (TMQ_TYPE -1: int8), or a refusal."""
+    code = types.get(x.dtype) if isinstance(x, torch.Tensor) else None
+    if code is None or not x.is_cuda or x.dim() != 2:
+        _refuse_rows(name, x, types)
+    M, K = x.shape
+    if K == 0 or K > k_max:
+        _refuse_rows(name, x, types)
+    return code, M, K, x.device
 
 
 def _unit_rows(x, M, K):
     """(tensor, row stride) with unit column stride and rows that do not overlap."""
-    if M == 1:
-        return x if K == 1 or x.stride(1) == 1 else x.contiguous(), (K + 15) // 16 * 16
-    if (x.stride(1) != 1 and K > 1) or x.stride(0) < K:
+    ld, step = x.stride()
+    if step != 1 and K > 1:
         x = x.contiguous()
-    return x, x.stride(0)
+        ld = K
+    if M == 1:
+        return x, (K + 15) // 16 * 16
+    if ld < K:
+        x = x.contiguous()
+        ld = K
+    return x, ld
 
 
 def _aligned_rows(x, M, K):
     """(tensor, row stride) of rows the TMA path can read: unit column stride, 16-byte aligned rows that do not overlap.
     Anything else is copied into such rows first."""
     lanes = 16 // x.element_size()
-    if (x.stride(1) == 1 or K == 1) and x.data_ptr() % 16 == 0:
+    ld, step = x.stride()
+    if (step == 1 or K == 1) and x.data_ptr() % 16 == 0:
         if M == 1:
             return x, (K + lanes - 1) // lanes * lanes
-        ld = x.stride(0)
         if ld >= K and ld % lanes == 0:
             return x, ld
     kp = (K + lanes - 1) // lanes * lanes
@@ -832,18 +848,16 @@ def _rows_out(name, out, M, N, dtype, device):
 
 
 def _code_scratch(code, M, K, device):
-    """Scratch for the codes and scales of floating-point activations (None for int8): stream-ordered caching allocator."""
-    if code < 0:
-        return None
-    n = lib().tmq_a8_workspace_bytes(code, M, K)
-    return torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device)
+    """Scratch for the codes and scales of floating-point activations: stream-ordered caching allocator."""
+    return torch.empty_strided((lib().tmq_a8_workspace_bytes(code, M, K),), (1,), dtype=torch.uint8, device=device)
 
 
-def _check_packed(name, wt, N, K, fmt, device):
+def _check_packed(name, wt, shape, K, fmt, device):
+    """wt: int32 tensor of `shape` (all but the last dimension) rows of prepacked words."""
     words = _row_words.get((K, fmt))
     if words is None:
         words = _row_words[(K, fmt)] = prepack_row_words(K, fmt)
-    if wt.dtype is not torch.int32 or wt.shape[-2:] != (N, words) or not wt.is_contiguous() or wt.device != device:
+    if wt.shape != shape + (words,) or wt.dtype is not torch.int32 or wt.device != device or not wt.is_contiguous():
         raise RuntimeError(f"{name}: prepacked weights do not match the problem's shape, kind or device")
 
 
@@ -854,13 +868,12 @@ def quantize_rows(x, out=None):
     rows padded to a multiple of 16 bytes, the form the 8-bit products read in place.  The rows of a weight matrix are its
     output channels: quantize_rows(weight) makes the operands of gemm_i8.  out: optional (codes, scale) to write into, codes
     with unit column stride; padding columns of `out` are not touched.  No gradient."""
-    code = _rows_type("quantize_rows", x, _TYPES)
-    M, K = x.shape
-    dev = x.device
+    code, M, K, dev = _rows_in("quantize_rows", x, _TYPES, 1 << 40)
     if out is None:
-        kp = width = ldq = (K + 15) // 16 * 16
-        q = torch.empty_strided((M, K), (kp, 1), dtype=torch.int8, device=dev) if kp == K else \
-            torch.empty_strided((M, kp), (kp, 1), dtype=torch.int8, device=dev)[:, :K]
+        width = ldq = (K + 15) // 16 * 16
+        q = torch.empty_strided((M, width), (width, 1), dtype=torch.int8, device=dev)
+        if width != K:
+            q = q.as_strided((M, K), (width, 1))
         scale = torch.empty_strided((M,), (1,), dtype=torch.float32, device=dev)
     else:
         q, scale = out
@@ -873,12 +886,8 @@ def quantize_rows(x, out=None):
     if M:
         x, ldx = _unit_rows(x, M, K)
         index = dev.index
-        args = (x.data_ptr(), code, q.data_ptr(), scale.data_ptr(), M, K, ldx, ldq, width)
-        if torch.cuda.current_device() == index:
-            rc = lib().tmq_quantize_rows(*args, torch._C._cuda_getCurrentRawStream(index))
-        else:
-            with torch.cuda.device(index):
-                rc = lib().tmq_quantize_rows(*args, torch._C._cuda_getCurrentRawStream(index))
+        rc = _enqueue(lib().tmq_quantize_rows, index, (x.data_ptr(), code, q.data_ptr(), scale.data_ptr(), M, K, ldx, ldq, width,
+                                                       _raw_stream(index)))
         if rc:
             check(rc, "quantize_rows")
     return q, scale
@@ -888,39 +897,41 @@ def ternary_gemm_a8(x, wt, columns, row_scale=None, scale=None, bias=None, out_d
     """Y[m][n] = row_scale[m] * scale[n] * sum_k x[m][k] T[n][k] + bias[n] with 8-bit activations and packed ternary
     weights; the sums are exact, the scaling is fp32, the result bf16, fp16 or fp32 [M, columns].
     x: CUDA int8 [M, K] (any row stride; row_scale fp32 [M] or None for 1), or fp32 / bf16 / fp16 [M, K], which is quantised
-    here exactly as quantize_rows does (inside the product's launch for a few rows).  wt: prepack(..., FMT_I8).
-    scale, bias: fp32 [columns] or None.  out: optional [M, columns] tensor of the output dtype whose rows may be strided.
-    No gradient."""
+    here exactly as quantize_rows does (inside the product's launch for a few rows).  wt: prepack(..., FMT_I8) (its rows are
+    padded, so a width close to the weights' own is not told apart from it).  scale, bias: fp32 [columns] or None.  out:
+    optional [M, columns] tensor of the output dtype whose rows may be strided.  No gradient."""
     name = "ternary_gemm_a8"
-    code = _rows_type(name, x, _A8_TYPES)
-    if code >= 0 and row_scale is not None:
-        raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
-    M, K = x.shape
-    if K > I8_K_MAX:
-        raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
+    code, M, K, dev = _rows_in(name, x, _A8_TYPES)
     N = int(columns)
-    dev = x.device
-    _check_packed(name, wt, N, K, FMT_I8, dev)
-    if wt.dim() != 2:
-        raise RuntimeError(f"{name}: expected the prepacked weights of one matrix")
-    rs, p_rs = _vector(name, "row_scale", row_scale, (M,), dev)
-    sc, p_sc = _vector(name, "scale", scale, (N,), dev)
-    bi, p_bi = _vector(name, "bias", bias, (N,), dev)
+    _check_packed(name, wt, (N,), K, FMT_I8, dev)
+    p_rs = p_sc = p_bi = p_ws = None
+    if row_scale is not None:
+        if code >= 0:
+            raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
+        row_scale = _vector(name, "row_scale", row_scale, (M,), dev)
+        p_rs = row_scale.data_ptr()
+    if scale is not None:
+        scale = _vector(name, "scale", scale, (N,), dev)
+        p_sc = scale.data_ptr()
+    if bias is not None:
+        bias = _vector(name, "bias", bias, (N,), dev)
+        p_bi = bias.data_ptr()
     y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
     x, ldx = _aligned_rows(x, M, K) if code < 0 else _unit_rows(x, M, K)
-    ws, nbytes, p_ws = None, 0, None
-    if M > A8_TOKENS or M * K > A8_FUSED_ELEMS:
+    ws, nbytes = None, 0
+    if code >= 0 and (M > A8_TOKENS or M * K > A8_FUSED_ELEMS):
         ws = _code_scratch(code, M, K, dev)
-    if ws is not None:
         nbytes, p_ws = ws.numel(), ws.data_ptr()
-    rc = _enqueue(lib().tmq_ternary_gemm_a8, dev.index, x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi, y.data_ptr(),
-                  y_code, M, N, K, ldy, p_ws, nbytes)
+    index = dev.index
+    fn, word, stream = lib().tmq_ternary_gemm_a8, _status_address.get(index) or _status_word_address(index), _raw_stream(index)
+    rc = _enqueue(fn, index, (x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi, y.data_ptr(), y_code, M, N, K, ldy, p_ws,
+                              nbytes, word, stream))
     if rc == -5:               # few rows, but a matrix whose share per SM exceeds its shared memory: not one launch
         ws = _code_scratch(code, M, K, dev)
-        rc = _enqueue(lib().tmq_ternary_gemm_a8, dev.index, x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi,
-                      y.data_ptr(), y_code, M, N, K, ldy, ws.data_ptr(), ws.numel())
+        rc = _enqueue(fn, index, (x.data_ptr(), code, ldx, p_rs, wt.data_ptr(), p_sc, p_bi, y.data_ptr(), y_code, M, N, K, ldy,
+                                  ws.data_ptr(), ws.numel(), word, stream))
     if rc:
         check(rc, name)
     _launched(dev)
@@ -949,27 +960,35 @@ def gemm_i8(x, weight, row_scale=None, scale=None, bias=None, out_dtype=torch.bf
     """ternary_gemm_a8 for 8-bit weights: weight int8 [N, K] with rows that start at multiples of 16 bytes (what
     quantize_rows returns), scale fp32 [N] per channel.  Everything else as there."""
     name = "gemm_i8"
-    code = _rows_type(name, x, _A8_TYPES)
-    if code >= 0 and row_scale is not None:
-        raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
-    M, K = x.shape
-    if K > I8_K_MAX:
-        raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
-    dev = x.device
+    code, M, K, dev = _rows_in(name, x, _A8_TYPES)
     ldw = _check_i8_weights(name, weight, 2, dev)
-    N = weight.shape[0]
-    if weight.shape[1] != K:
+    N, width = weight.shape
+    if width != K:
         raise RuntimeError(f"{name}: activation width does not match the weights")
-    rs, p_rs = _vector(name, "row_scale", row_scale, (M,), dev)
-    sc, p_sc = _vector(name, "scale", scale, (N,), dev)
-    bi, p_bi = _vector(name, "bias", bias, (N,), dev)
+    p_rs = p_sc = p_bi = p_ws = None
+    if row_scale is not None:
+        if code >= 0:
+            raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
+        row_scale = _vector(name, "row_scale", row_scale, (M,), dev)
+        p_rs = row_scale.data_ptr()
+    if scale is not None:
+        scale = _vector(name, "scale", scale, (N,), dev)
+        p_sc = scale.data_ptr()
+    if bias is not None:
+        bias = _vector(name, "bias", bias, (N,), dev)
+        p_bi = bias.data_ptr()
     y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
     x, ldx = _aligned_rows(x, M, K) if code < 0 else _unit_rows(x, M, K)
-    ws = _code_scratch(code, M, K, dev)
-    rc = _enqueue(lib().tmq_gemm_i8, dev.index, x.data_ptr(), code, ldx, p_rs, weight.data_ptr(), ldw, p_sc, p_bi, y.data_ptr(),
-                  y_code, M, N, K, ldy, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+    nbytes = 0
+    if code >= 0:
+        ws = _code_scratch(code, M, K, dev)
+        nbytes, p_ws = ws.numel(), ws.data_ptr()
+    index = dev.index
+    rc = _enqueue(lib().tmq_gemm_i8, index, (x.data_ptr(), code, ldx, p_rs, weight.data_ptr(), ldw, p_sc, p_bi, y.data_ptr(),
+                                             y_code, M, N, K, ldy, p_ws, nbytes,
+                                             _status_address.get(index) or _status_word_address(index), _raw_stream(index)))
     if rc:
         check(rc, name)
     _launched(dev)
@@ -977,12 +996,21 @@ def gemm_i8(x, weight, row_scale=None, scale=None, bias=None, out_dtype=torch.bf
 
 
 def _check_offsets(name, offsets, groups, device):
-    if offsets.dtype not in (torch.int32, torch.int64) or offsets.device != device or offsets.dim() != 1 or \
-            offsets.shape[0] != groups + 1 or not offsets.is_contiguous():
+    if offsets.dtype not in (torch.int32, torch.int64) or offsets.device != device or offsets.shape != (groups + 1,) or \
+            not offsets.is_contiguous():
         raise RuntimeError(f"{name}: offsets must be a contiguous int32 or int64 tensor of experts + 1 boundaries on the "
                            "activations' device")
     if not 1 <= groups <= GROUPS_MAX:
         raise RuntimeError(f"{name}: 1 .. {GROUPS_MAX} experts")
+
+
+def _grouped_tables(name, E, N, M, row_scale, scales, biases, device):
+    """The optional fp32 tables of a grouped product (kept by the caller until the launch) and their addresses."""
+    row_scale = None if row_scale is None else _vector(name, "row_scale", row_scale, (M,), device)
+    scales = None if scales is None else _vector(name, "scales", scales, (E, N), device)
+    biases = None if biases is None else _vector(name, "biases", biases, (E, N), device)
+    keep = (row_scale, scales, biases)
+    return keep, [None if t is None else t.data_ptr() for t in keep]
 
 
 def ternary_gemm_grouped(x, wts, columns, offsets, row_scale=None, scales=None, biases=None, out_dtype=torch.bfloat16,
@@ -996,32 +1024,29 @@ def ternary_gemm_grouped(x, wts, columns, offsets, row_scale=None, scales=None, 
     fresh result and left as they were in `out`.  Boundaries outside 0 .. M or out of order give empty or shortened groups.
     No gradient."""
     name = "ternary_gemm_grouped"
-    i8 = _rows_type(name, x, _GROUPED_TYPES) < 0
-    M, K = x.shape
+    code, M, K, dev = _rows_in(name, x, _GROUPED_TYPES, 1 << 40)
+    if code < 0 and K > I8_K_MAX:
+        _refuse_rows(name, x, _GROUPED_TYPES)
     N = int(columns)
-    dev = x.device
     if not isinstance(wts, torch.Tensor) or wts.dim() != 3:
         raise RuntimeError(f"{name}: expected the stacked prepacked weights [experts, columns, row words]")
     E = wts.shape[0]
     _check_offsets(name, offsets, E, dev)
-    _check_packed(name, wts, N, K, FMT_I8 if i8 else FMT_BF16, dev)
-    if i8 and K > I8_K_MAX:
-        raise RuntimeError(f"{name}: at most {I8_K_MAX} columns (int32 sums)")
-    if not i8 and row_scale is not None:
+    _check_packed(name, wts, (E, N), K, FMT_I8 if code < 0 else FMT_BF16, dev)
+    if code >= 0 and row_scale is not None:
         raise RuntimeError(f"{name}: row_scale belongs to int8 activations")
-    rs, p_rs = _vector(name, "row_scale", row_scale, (M,), dev)
-    sc, p_sc = _vector(name, "scales", scales, (E, N), dev)
-    bi, p_bi = _vector(name, "biases", biases, (E, N), dev)
+    keep, (p_rs, p_sc, p_bi) = _grouped_tables(name, E, N, M, row_scale, scales, biases, dev)
     y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
     x, ldx = _aligned_rows(x, M, K)
+    index = dev.index
     tail = (wts.data_ptr(), p_sc, p_bi, offsets.data_ptr(), offsets.element_size(), E, y.data_ptr(), y_code, M, N, K, ldy,
-            1 if out is None else 0)
-    if i8:
-        rc = _enqueue(lib().tmq_ternary_gemm_grouped_a8, dev.index, x.data_ptr(), ldx, p_rs, *tail)
+            1 if out is None else 0, _status_address.get(index) or _status_word_address(index), _raw_stream(index))
+    if code < 0:
+        rc = _enqueue(lib().tmq_ternary_gemm_grouped_a8, index, (x.data_ptr(), ldx, p_rs) + tail)
     else:
-        rc = _enqueue(lib().tmq_ternary_gemm_grouped_bf16, dev.index, x.data_ptr(), ldx, *tail)
+        rc = _enqueue(lib().tmq_ternary_gemm_grouped_bf16, index, (x.data_ptr(), ldx) + tail)
     if rc:
         check(rc, name)
     _launched(dev)
@@ -1032,23 +1057,22 @@ def gemm_i8_grouped(x, weights, offsets, row_scale=None, scales=None, biases=Non
     """ternary_gemm_grouped for 8-bit weights: weights int8 [experts, N, K] whose rows lie one behind the other and start at
     multiples of 16 bytes; x int8 [M, K] with row_scale fp32 [M].  Everything else as there."""
     name = "gemm_i8_grouped"
-    _rows_type(name, x, _I8_TYPES)
-    M, K = x.shape
-    dev = x.device
+    _, M, K, dev = _rows_in(name, x, _I8_TYPES)
     ldw = _check_i8_weights(name, weights, 3, dev)
-    E, N = weights.shape[:2]
+    E, N, width = weights.shape
     _check_offsets(name, offsets, E, dev)
-    if weights.shape[2] != K or K > I8_K_MAX:
-        raise RuntimeError(f"{name}: activation width does not match the weights or exceeds the int32 sums")
-    rs, p_rs = _vector(name, "row_scale", row_scale, (M,), dev)
-    sc, p_sc = _vector(name, "scales", scales, (E, N), dev)
-    bi, p_bi = _vector(name, "biases", biases, (E, N), dev)
+    if width != K:
+        raise RuntimeError(f"{name}: activation width does not match the weights")
+    keep, (p_rs, p_sc, p_bi) = _grouped_tables(name, E, N, M, row_scale, scales, biases, dev)
     y, ldy, y_code = _rows_out(name, out, M, N, out_dtype, dev)
     if M == 0:
         return y
     x, ldx = _aligned_rows(x, M, K)
-    rc = _enqueue(lib().tmq_gemm_grouped_i8, dev.index, x.data_ptr(), ldx, p_rs, weights.data_ptr(), ldw, p_sc, p_bi,
-                  offsets.data_ptr(), offsets.element_size(), E, y.data_ptr(), y_code, M, N, K, ldy, 1 if out is None else 0)
+    index = dev.index
+    rc = _enqueue(lib().tmq_gemm_grouped_i8, index, (
+        x.data_ptr(), ldx, p_rs, weights.data_ptr(), ldw, p_sc, p_bi, offsets.data_ptr(), offsets.element_size(), E,
+        y.data_ptr(), y_code, M, N, K, ldy, 1 if out is None else 0, _status_address.get(index) or _status_word_address(index),
+        _raw_stream(index)))
     if rc:
         check(rc, name)
     _launched(dev)
