@@ -71,6 +71,8 @@ def test_linear_with_8_bit_activations(tmq, dtype, post_scale):
         ref = want(x2, w, lin.post_scale_imm, lin.bias.detach().cpu())
         q, s = row_codes(x2)
         close(y.reshape(-1, 77), ref, (q.abs() @ w.abs().double().t()) * s * abs(lin.post_scale_imm))
+    with pytest.raises(RuntimeError):
+        lin(torch.ones(2, 204, device="cuda", dtype=dtype))
     raw = lin(torch.ones(2, 203, dtype=torch.int8, device="cuda"))          # codes keep their raw sums
     assert raw.dtype == torch.int32
     tmq.set_activation_bits(holder, None)

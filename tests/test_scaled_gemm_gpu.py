@@ -238,7 +238,7 @@ GROUPS = [[5], [0, 3], [1, 1, 1, 1], [0, 0, 0], [64, 0, 65, 1], [7, 300, 0, 2], 
 
 
 @pytest.mark.parametrize("form", ["ternary_i8", "ternary_bf16", "int8"])
-@pytest.mark.parametrize("N,K", [(130, 72), (256, 1040), (33, 200)])
+@pytest.mark.parametrize("N,K", [(130, 72), (256, 1040), (33, 200), (130, 128), (200, 640), (64, 64)])
 @pytest.mark.parametrize("counts", GROUPS, ids=lambda c: f"{len(c)}x{sum(c)}")
 def test_grouped(ops, counts, N, K, form):
     E, T = len(counts), sum(counts)

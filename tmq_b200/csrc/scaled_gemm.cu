@@ -5,17 +5,20 @@
 //
 //   * A work unit is (expert, up to BN of its rows, 128 channels).  The weight tile is the 128-row "A" operand, the rows
 //     are the N side of the MMA, so a decoded weight tile serves up to BN rows, and the N of a unit's MMAs is its row
-//     count rounded up to 32: an expert with three rows costs 32 columns of tensor work and 32 rows of operand traffic
-//     whatever BN is.
+//     count rounded up to 32.
 //   * The group boundaries stay on the device.  Every CTA scans them into a table of tile counts in shared memory
 //     (clamped to the rows that exist and made non-decreasing: bad boundaries give empty groups, never a bad address) and
-//     walks the units u = CTA, CTA + grid, ... through it.
+//     takes every gridDim.x-th unit of it.
 //   * Roles: warp 0 TMA of the activations (and 8-bit weights), warp 1 MMA issue, warp 2 TMA of the packed weights, then
-//     decode warps (packed weights only) and epilogue warps.  Decoded
-//     weights go to tensor memory (the MMA reads its A operand there) except for int8 tiles of 256 rows, whose two
-//     accumulators fill tensor memory: those are decoded into shared memory.  8-bit weights need no decode, TMA writes
-//     them where the MMA reads them.
+//     decode warps (packed weights only) and epilogue warps.  Decoded weights go to tensor memory (the MMA reads its A
+//     operand there) except for int8 tiles of 256 rows, whose two accumulators fill tensor memory: those are decoded into
+//     shared memory.  8-bit weights need no decode, TMA writes them where the MMA reads them.
 //   * Every wait is bounded (TMQ_ERR_TIMEOUT in the status word).
+//
+// What bounds it: tall tiles the tensor pipe (bf16 256 rows: 510 cycles per k-block, 512 of MMA; int8 256 rows: shared-memory
+// bandwidth, 104 KB per k-block), under the power cap 8192 x 28672 x 8192 int8 in 1.37 ms = 2.8 Pop/s; 8-bit weights and few
+// rows memory (28672 x 8192, up to 32 rows: 40 us = 5.9 TB/s); ternary weights and few rows the issue of small MMAs (about 48
+// cycles each) and the decoding (140 cycles of the integer pipe per 16 K codes), 137 ns per k-block against 93 of memory.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -54,7 +57,8 @@ struct ScaledCfg {
     static constexpr int RAWK = DENSE ? 1 : (TA ? 4 : 2);
     static constexpr int RAW_PITCH = RAWK * RAW_ROW;
     // A pipeline stage is KB k-blocks: the MMA warp pays its barrier round (about 270 cycles of latency) once a stage, and
-    // four MMAs of a k-block alone cover 170.  One k-block per stage measured 280 - 300 ns per k-block for every BN <= 128.
+    // four MMAs of a k-block alone cover 170.  One k-block per stage measured 280 - 300 ns per k-block for every BN <= 128; two
+    // instead of four for tiles of up to 64 rows 199 instead of 174 (32 rows, k-blocks of K = 16384 with fill and drain).
     static constexpr int KB = !TA && BN > 128 ? 1 : (TA && BN <= 64) ? 4 : 2;
     // Three rings: decoded weights (NA stages; tensor memory, or shared memory for int8 tiles of 256 rows), activations and
     // 8-bit weights (NB stages), packed words (RAW_STAGES boxes).  An activation box takes about 1250 cycles from L2, so its
@@ -244,10 +248,10 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                     if (++s == C::NB) { s = 0; ph ^= 1u; round = 1; }
                 }
             }
-            // gave up: wait for the copies still on their way (ph: parity of this round's slots waiting to be refilled)
-            if (!ok)
-                for (int i = 0; i < C::NB; i++)
-                    if (round || i < s) ptx::mbar_wait_own(full + i, i < s ? ph ^ 1u : ph, a.status);
+            // no copy may be on its way when the CTA ends, whatever became of the others (ph: parity of the slots that this
+            // round has yet to refill)
+            for (int i = 0; i < C::NB; i++)
+                if (round || i < s) ptx::mbar_wait_own(full + i, i < s ? ph ^ 1u : ph, a.status);
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer (whole warp walks, one lane issues)
@@ -333,9 +337,8 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                     if (++s == C::RAW_STAGES) { s = 0; ph ^= 1u; round = 1; }
                 }
             }
-            if (!ok)
-                for (int i = 0; i < C::RAW_STAGES; i++)
-                    if (round || i < s) ptx::mbar_wait_own(raw_full + i, i < s ? ph ^ 1u : ph, a.status);
+            for (int i = 0; i < C::RAW_STAGES; i++)
+                if (round || i < s) ptx::mbar_wait_own(raw_full + i, i < s ? ph ^ 1u : ph, a.status);
         }
     } else if (!C::DENSE && warp >= 4 && warp < C::FIRST_EPI) {
         // ---------------------------------------------------------------- decode

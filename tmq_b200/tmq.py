@@ -535,6 +535,8 @@ class TMQLayer:
 class Linear(nn.Module, TMQLayer):
     """Quantization-aware drop-in for nn.Linear [tmq/tmq.py:573-765]."""
 
+    activation_bits = None      # precision of the activations in compact inference (set_activation_bits)
+
     def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None,
                  ctrl: QuantizationControl = None, quant_mode=QuantMode.NONE, post_scale=False):
         super(Linear, self).__init__()
@@ -547,7 +549,6 @@ class Linear(nn.Module, TMQLayer):
         self.post_scale_imm = 1.0 / (self._in_features * self._variance_estimate()) if post_scale else 1.0
         self.post_scale = nn.Parameter(torch.tensor(self.post_scale_imm), requires_grad=False)
         self.bn = None
-        self.activation_bits = None
 
     def __repr__(self):
         if len(self.original_shape) == 2:
@@ -597,6 +598,8 @@ class Linear(nn.Module, TMQLayer):
         x2d = x.reshape(-1, x.shape[-1])
         if self.activation_bits == 8 and x.dtype != torch.int8:
             n_out = self._gemm_columns()
+            if x2d.shape[1] != int(self.original_shape[1]):
+                raise RuntimeError("compact inference: activation width does not match the packed weights")
             out = ops.ternary_gemm_a8(x2d, self._prepacked_weights(ops.FMT_I8), n_out, scale=self._channel_scale(n_out, x.device),
                                       bias=self.bias, out_dtype=x.dtype)
         else:
