@@ -22,9 +22,10 @@ struct QuantArgs {
     int vstore;
 };
 
-// One row per TPR threads, 256 threads per block, CH vectors held per thread; the rest of a longer row is read twice.
+// One row per TPR threads, 256 threads per block, CH vectors held per thread; the rest of a longer row is read twice.  Six
+// blocks per SM where their registers allow it (8192 x 8192 bf16: 36.3 us, 5.5 TB/s, against 37.5 with five and 40 with seven).
 template <typename T, bool VLOAD, int TPR, int CH>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(256, VLOAD && CH <= 4 ? 6 : 1) quantize_rows_kernel(const QuantArgs a) {
     constexpr int ROWS = 256 / TPR, V = QuantType<T>::V;
     __shared__ uint32_t red[8];
     asm volatile("griddepcontrol.wait;" ::: "memory");
