@@ -23,9 +23,10 @@ struct QuantArgs {
 };
 
 // One row per TPR threads, 256 threads per block, CH vectors held per thread; the rest of a longer row is read twice.  Six
-// blocks per SM where their registers allow it (8192 x 8192 bf16: 36.3 us, 5.5 TB/s, against 37.5 with five and 40 with seven).
+// blocks per SM where their registers allow it (8192 x 8192 bf16: 36.3 us, 5.5 TB/s, against 37.5 with five and 40 with seven),
+// four for the others (1037 x 5003 fp32 rows without alignment: 7.6 us, 9.0 with more registers and fewer blocks).
 template <typename T, bool VLOAD, int TPR, int CH>
-__global__ void __launch_bounds__(256, VLOAD && CH <= 4 ? 6 : 1) quantize_rows_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(256, VLOAD && CH <= 4 ? 6 : sizeof(T) == 2 && !VLOAD && CH > 4 ? 3 : 4) quantize_rows_kernel(const QuantArgs a) {
     constexpr int ROWS = 256 / TPR, V = QuantType<T>::V;
     __shared__ uint32_t red[8];
     asm volatile("griddepcontrol.wait;" ::: "memory");
