@@ -10,13 +10,12 @@
 //     (clamped to the rows that exist and made non-decreasing: bad boundaries give empty groups, never a bad address) and
 //     takes every gridDim.x-th unit of it.
 //   * Roles: warp 0 TMA of the activations (and 8-bit weights), warp 1 MMA issue, warp 2 TMA of the packed weights, then
-//     decode warps (packed weights only) and epilogue warps.  Decoded weights go to tensor memory (the MMA reads its A
-//     operand there) except for int8 tiles of 256 rows, whose two accumulators fill tensor memory: those are decoded into
-//     shared memory.  8-bit weights need no decode, TMA writes them where the MMA reads them.
+//     decode warps (packed weights only) and epilogue warps.  Decoded weights go to tensor memory, where the MMA reads its A
+//     operand without a byte through shared memory; 8-bit weights need no decode, TMA writes them where the MMA reads them.
 //   * Every wait is bounded (TMQ_ERR_TIMEOUT in the status word).
 //
-// What bounds it: tall tiles the tensor pipe (bf16 256 rows: 510 cycles per k-block, 512 of MMA; int8 256 rows: shared-memory
-// bandwidth, 104 KB per k-block), under the power cap 8192 x 28672 x 8192 int8 in 1.37 ms = 2.8 Pop/s; 8-bit weights and few
+// What bounds it: tall tiles the tensor pipe (bf16 256 rows: 510 cycles per k-block, 512 of them MMA) and 8-bit weights shared
+// memory (96 KB per k-block), int8 8192 x 28672 x 8192 in 1.24 ms = 3.1 Pop/s; 8-bit weights and few
 // rows memory (28672 x 8192, up to 32 rows: 40 us = 5.9 TB/s); ternary weights and few rows the issue of small MMAs (about 48
 // cycles each) and the decoding (140 cycles of the integer pipe per 16 K codes), 137 ns per k-block against 93 of memory.
 #include <cuda.h>
@@ -48,28 +47,32 @@ struct ScaledMaps {
 template <int WK, int BN>
 struct ScaledCfg {
     static constexpr bool DENSE = WK == W_DENSE_I8, I8 = WK != W_TERNARY_BF16;
-    static constexpr bool TA = WK == W_TERNARY_BF16 || (WK == W_TERNARY_I8 && BN <= 128);   // A operand in tensor memory
+    static constexpr bool TA = !DENSE;                                        // A operand in tensor memory
     static constexpr int BK = I8 ? 128 : 64;
     static constexpr int RAW_ROW = DENSE ? 0 : I8 ? 32 : 16;                  // packed bytes per channel and k-block
     // Packed words come RAWK k-blocks per box: a box costs the TMA unit about four cycles a row whatever its width (one
     // k-block per box measured 280 ns per k-block at any row count).  Rows of 128 / 64 bytes with the swizzle of that
-    // width, so the decode warps' 16-byte reads meet no bank conflicts.
-    static constexpr int RAWK = DENSE ? 1 : (TA ? 4 : 2);
+    // width, so the decode warps' 16-byte reads meet no bank conflicts.  (Two k-blocks for int8 tiles of 256 rows, whose
+    // activations take 192 KB.)
+    static constexpr int RAWK = DENSE ? 1 : I8 && BN > 128 ? 2 : 4;
     static constexpr int RAW_PITCH = RAWK * RAW_ROW;
     // A pipeline stage is KB k-blocks: the MMA warp pays its barrier round (about 270 cycles of latency) once a stage, and
     // four MMAs of a k-block alone cover 170.  One k-block per stage measured 280 - 300 ns per k-block for every BN <= 128; two
     // instead of four for tiles of up to 64 rows 199 instead of 174 (32 rows, k-blocks of K = 16384 with fill and drain).
-    static constexpr int KB = !TA && BN > 128 ? 1 : (TA && BN <= 64) ? 4 : 2;
-    // Three rings: decoded weights (NA stages; tensor memory, or shared memory for int8 tiles of 256 rows), activations and
+    static constexpr int KB = DENSE && BN > 128 ? 1 : !DENSE && BN <= 64 ? 4 : 2;
+    // Three rings: decoded weights (NA stages of tensor memory), activations and
     // 8-bit weights (NB stages), packed words (RAW_STAGES boxes).  An activation box takes about 1250 cycles from L2, so its
     // ring is the one that must be deep: three stages of four k-blocks, shared with the weights, held bf16 tiles of 64 rows
     // at 154 ns per k-block.
-    static constexpr int NA = DENSE ? 0 : !TA ? 4 : BN > 128 ? 3 : BN > 64 ? 4 : 3;
-    static constexpr int NB = DENSE ? (BN > 128 ? 4 : BN > 64 ? 3 : BN > 32 ? 4 : 5) : !TA ? 4 : BN > 128 ? 3 : BN > 64 ? 5 : BN > 32 ? 4 : 7;
-    static constexpr int RAW_STAGES = DENSE ? 0 : !TA ? 2 : BN > 128 ? 2 : BN > 64 ? 3 : 4;
-    static constexpr int A_BYTES = TA ? 0 : kTileC * kOpRow;                     // of one k-block
+    static constexpr int NA = DENSE ? 0 : BN > 128 ? (I8 ? 4 : 3) : BN > 64 ? 4 : 3;
+    static constexpr int NB = DENSE ? (BN > 128 ? 4 : BN > 64 ? 3 : BN > 32 ? 4 : 5) : BN > 128 ? 3 : BN > 64 ? 5 : BN > 32 ? 4 : 7;
+    static constexpr int RAW_STAGES = DENSE ? 0 : BN > 128 ? 2 : BN > 64 ? 3 : 4;
+    static constexpr int A_BYTES = TA ? 0 : kTileC * kOpRow;                  // of one k-block
     static constexpr int B_BYTES = BN * kOpRow;
     static constexpr int RAW_BYTES = kTileC * RAW_PITCH;
+    // Two accumulators, so that one unit's results leave under the next unit's MMAs, but one where 256 rows and the decoded
+    // weights fill tensor memory.  (int8 with two accumulators and the weights decoded into shared memory, 104 KB a k-block
+    // through it: 8192 x 28672 x 8192 1375 us, against 1240.)
     static constexpr int ACC_BUFS = (TA && BN > 128) ? 1 : 2;
     static constexpr int A_COLS = kOpRow / 4;
     static constexpr int A_BASE = ACC_BUFS * BN;
@@ -84,11 +87,10 @@ struct ScaledCfg {
     static constexpr int DECODERS = DENSE ? 0 : 4 * SETS;
     static constexpr int FIRST_EPI = 4 + DECODERS;
     static constexpr int EPI = BN > 128 ? 8 : 4;                              // epilogue warps
-    static constexpr int READY = KB == 1 ? 4 : 8;                             // warps that decode one stage
     static constexpr int THREADS = (FIRST_EPI + EPI) * 32;
     // shared memory
     static constexpr int A_OFF = 0;
-    static constexpr int B_OFF = A_OFF + (DENSE ? NB : NA) * KB * A_BYTES;
+    static constexpr int B_OFF = A_OFF + NB * KB * A_BYTES;
     static constexpr int RAW_OFF = B_OFF + NB * KB * B_BYTES;
     static constexpr int RS_OFF = RAW_OFF + RAW_STAGES * RAW_BYTES;           // 32 row scales per epilogue warp
     static constexpr int BAR_OFF = RS_OFF + EPI * 128;
@@ -185,7 +187,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             ptx::mbar_init(empty + s, 1);
         }
         for (int s = 0; s < C::NA; s++) {
-            ptx::mbar_init(ready + s, C::READY);
+            ptx::mbar_init(ready + s, 8);
             ptx::mbar_init(taken + s, 1);
         }
         for (int s = 0; s < C::RAW_STAGES; s++) {
@@ -277,7 +279,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                     if (!landed) ok = ptx::mbar_wait_warp(acts ? full + sb : ready + sa, acts ? pb : pa, a.status);
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
-                    const uint64_t a_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::A_OFF + (C::DENSE ? sb : sa) * C::KB * C::A_BYTES));
+                    const uint64_t a_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::A_OFF + sb * C::KB * C::A_BYTES));
                     const uint64_t b_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::B_OFF + sb * C::KB * C::B_BYTES));
                     const uint32_t a_tmem = tmem_base + C::A_BASE + (uint32_t)(sa * C::KB * C::A_COLS);
                     uint64_t *const used_a = taken + sa, *const used_b = empty + sb;
@@ -346,7 +348,6 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         const int row = quarter * 32 + lane;
         const uint32_t raw_row = ptx::smem_u32(smem + C::RAW_OFF) + (uint32_t)(row * C::RAW_PITCH);
         const uint32_t swz = (uint32_t)(C::RAW_PITCH == 128 ? row & 7 : (row >> 1) & 3) << 4;
-        const uint32_t a_row = ptx::smem_u32(smem + C::A_OFF) + (uint32_t)(row * kOpRow);
         const uint32_t a_lane = tmem_base + ((uint32_t)(quarter * 32) << 16) + C::A_BASE;
         const uint32_t ready0 = ptx::smem_u32(ready), taken0 = ptx::smem_u32(taken), raw_full0 = ptx::smem_u32(raw_full),
                        raw_empty0 = ptx::smem_u32(raw_empty);
@@ -359,19 +360,15 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
 #pragma unroll
                     for (int st = 0; st < C::RAWK; st += C::KB) {
                         if (st > 0 && st >= left) break;
-                        if (C::KB == 1 && st != half) {  // one k-block per stage: the other set's
-                            if (++s == C::NA) { s = 0; ph ^= 1u; }
-                            continue;
-                        }
                         // even lanes wait for the packed words, odd lanes for the slot; a set whose k-block lies beyond the
                         // unit waits (and reports) as well, or it would run a round ahead of the others
                         ok = ptx::mbar_wait_warp_at((lane & 1) ? taken0 + 8u * s : raw_full0 + 8u * rs, (lane & 1) ? ph : rph, a.status);
                         if (!ok) break;
-                        if (C::TA) ptx::tc_fence_after_sync();
+                        ptx::tc_fence_after_sync();
 #pragma unroll
                         for (int jj = 0; jj < (C::KB == 4 ? 2 : 1); jj++) {
                             // k-block of the box, and of the stage
-                            const int j = C::KB == 4 ? half + 2 * jj : C::KB == 2 ? st + half : st, js = C::KB == 1 ? 0 : j - st;
+                            const int j = C::KB == 4 ? half + 2 * jj : st + half, js = j - st;
                             if (j > 0 && j >= left) break;
                             const uint32_t words0 = raw_row + (uint32_t)(rs * C::RAW_BYTES);
                             uint32_t cols[32];           // the row's 128 operand bytes, K ascending
@@ -397,29 +394,15 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                                     for (int x = 0; x < 8; x++) cols[8 * wi + x] = d[x];
                                 }
                             }
-                            if (C::TA) {
-                                ptx::tmem_st_x32(a_lane + (uint32_t)((s * C::KB + js) * C::A_COLS), cols);
-                            } else {
-                                const uint32_t dst = a_row + (uint32_t)((s * C::KB + js) * C::A_BYTES);
-#pragma unroll
-                                for (int c = 0; c < 8; c++)
-                                    ptx::sts_v4(dst + (uint32_t)((c ^ (row & 7)) << 4), cols[4 * c], cols[4 * c + 1], cols[4 * c + 2],
-                                                cols[4 * c + 3]);
-                            }
+                            ptx::tmem_st_x32(a_lane + (uint32_t)((s * C::KB + js) * C::A_COLS), cols);
                         }
-                        if (C::TA) {
-                            ptx::tmem_st_wait();
-                            ptx::tc_fence_before_sync();
-                        } else {
-                            ptx::fence_proxy_async_smem();
-                        }
+                        ptx::tmem_st_wait();
+                        ptx::tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) ptx::mbar_arrive_at(ready0 + 8u * s);
                         if (++s == C::NA) { s = 0; ph ^= 1u; }
                     }
                     if (!ok) break;
-                    if (C::KB == 1 && half == 1 && left == 1)        // no stage of its own in this box: wait for it all the same
-                        ok = ptx::mbar_wait_warp_at(raw_full0 + 8u * rs, rph, a.status);
                     __syncwarp();
                     if (ok && lane == 0) ptx::mbar_arrive_at(raw_empty0 + 8u * rs);
                 } else {                                 // the other pair's box
