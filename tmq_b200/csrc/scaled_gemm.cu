@@ -543,8 +543,8 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
 // measured: 155 / 160 / 240 / 352 ns for 32 / 64 / 128 / 256 rows (int8 and bf16 alike within a sixth), 0.6 us more to fill and
 // drain per doubling.  The row tiles of experts are not known here: the even share plus 0.6 of a tile each.  Over 150 shapes
 // (48 .. 2048 rows, 1 .. 128 experts with 1 .. 512 rows each on average) the choice costs 1 % on average against the best
-// tile of each; e.g. 517 x 11008 x 4096 int8 52.6 / 35.3 / 27.9 / 30.5 us, 64 experts of 48 rows 58.6 / 45.1 / 47.9 / 68.0 us,
-// of 512 rows 438 / 250 / 202 / 184 us.
+// tile of each; e.g. 517 x 11008 x 4096 int8 53.0 / 35.3 / 27.8 / 28.5 us, 64 experts (2816 x 2048) of 40 rows 54.0 / 45.2 /
+// 46.6 / 60.8 us, of 512 rows 472 / 275 / 207 / 191 us.
 static int unit_rows(const ScaledArgs &a, int bk) {
     static const double per_block[4] = {0.155, 0.160, 0.240, 0.352};
     const double blocks = (double)((a.K + bk - 1) / bk), tiles_n = (double)((a.N + kTileC - 1) / kTileC);
