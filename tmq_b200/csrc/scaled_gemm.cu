@@ -16,8 +16,8 @@
 //
 // What bounds it: tall tiles the tensor pipe (bf16 256 rows: 510 cycles per k-block, 512 of them MMA) and 8-bit weights shared
 // memory (96 KB per k-block), int8 8192 x 28672 x 8192 in 1.24 ms = 3.1 Pop/s; 8-bit weights and few
-// rows memory (28672 x 8192, up to 32 rows: 40 us = 5.9 TB/s); ternary weights and few rows the issue of small MMAs (about 48
-// cycles each) and the decoding (140 cycles of the integer pipe per 16 K codes), 137 ns per k-block against 93 of memory.
+// rows memory (28672 x 8192, up to 32 rows: 40 us = 5.9 TB/s); ternary weights and few rows the decode warps' integer
+// instructions: 140 ns per k-block, of which 104 remain without the decoding and 92 without its stores, where memory's 93 are.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
