@@ -158,6 +158,14 @@ def test_products_from_codes(ops, M, N, K, dense):
     ops.check_gemm_status()
 
 
+@pytest.mark.parametrize("dense", [False, True])
+@pytest.mark.parametrize("M,N,K", [(710, 2024, 700), (900, 1700, 1500), (400, 14000, 700), (2404, 1058, 930), (517, 11008, 1100),
+                                   (1000, 11008, 300), (1747, 2100, 1007)])
+def test_products_with_rows_dealt_evenly(ops, M, N, K, dense):
+    """Sizes whose row tiles are neither 32, 64, 128 nor 256 rows high (80, 96, 112, 160, 176, 208, 224)."""
+    test_products_from_codes(ops, M, N, K, dense)
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("M,N,K", [(1, 11008, 4096), (1, 77, 5), (2, 300, 1027), (4, 1000, 8192), (5, 640, 512), (8, 129, 2051),
                                    (12, 500, 700), (40, 300, 260), (200, 260, 515)])

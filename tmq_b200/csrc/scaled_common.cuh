@@ -20,6 +20,7 @@ struct ScaledArgs {
     long long M, N, K, ldy;
     int groups, offsets64, y_type, zero_rest;
     int wide;                        // K is whole k-blocks: one box per stage
+    int unit_rows, row_tiles;        // rows of a work unit, row tiles of a plain product
     int rows_first;                  // order of the work units (plain product only)
     int *status;
 };
@@ -98,7 +99,7 @@ __device__ __forceinline__ void build_table(const ScaledArgs &a, int *begin, int
     if (!a.offsets) {
         if (lane == 0) {
             begin[0] = 0; begin[1] = (int)a.M;
-            tiles[0] = 0; tiles[1] = (int)((a.M + bn - 1) / bn);
+            tiles[0] = 0; tiles[1] = a.row_tiles;
         }
         return;
     }

@@ -5,7 +5,7 @@
 //
 //   * A work unit is (expert, up to BN of its rows, 128 channels).  The weight tile is the 128-row "A" operand, the rows
 //     are the N side of the MMA, so a decoded weight tile serves up to BN rows, and the N of a unit's MMAs is its row
-//     count rounded up to 32.
+//     count rounded up to 16.
 //   * The group boundaries stay on the device.  Every CTA scans them into a table of tile counts in shared memory
 //     (clamped to the rows that exist and made non-decreasing: bad boundaries give empty groups, never a bad address) and
 //     takes every gridDim.x-th unit of it.
@@ -14,7 +14,7 @@
 //     operand without a byte through shared memory; 8-bit weights need no decode, TMA writes them where the MMA reads them.
 //   * Every wait is bounded (TMQ_ERR_TIMEOUT in the status word).
 //
-// What bounds it: tall tiles the tensor pipe (bf16 256 rows: 510 cycles per k-block, 512 of them MMA) and 8-bit weights shared
+// What bounds it: tall tiles the tensor pipe (bf16 256 rows: the 512 cycles per k-block that its MMAs take) and 8-bit weights shared
 // memory (96 KB per k-block), int8 8192 x 28672 x 8192 in 1.24 ms = 3.1 Pop/s; 8-bit weights and few
 // rows memory (28672 x 8192, up to 32 rows: 40 us = 5.9 TB/s); ternary weights and few rows the decode warps' integer
 // instructions: 140 ns per k-block, of which 104 remain without the decoding and 92 without its stores, where memory's 93 are.
@@ -32,7 +32,7 @@ namespace tmq {
 
 constexpr int kTileC = 128;          // channels of a unit (MMA M)
 constexpr int kOpRow = 128;          // bytes of one operand row per k-block: 64 bf16 or 128 int8
-constexpr int kRowStep = 32;         // granularity of a unit's MMA N
+constexpr int kRowStep = 16;         // granularity of a unit's MMA N
 
 // Tensor maps of a launch.  A TMA instruction costs about 200 cycles of its unit whatever it brings (bf16 tiles of 32 rows
 // with one box per k-block: 154 ns per k-block), so a box spans all k-blocks of a stage where the row length allows it.
@@ -180,6 +180,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int nkb = (int)((a.K + C::BK - 1) / C::BK);
     const int tiles_n = (int)((a.N + kTileC - 1) / kTileC);
+    const int unit_rows = BN > 64 ? a.unit_rows : BN;        // (low tiles are never balanced)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < C::NB; s++) {
@@ -224,7 +225,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             uint32_t ph = 1;
             bool ok = true;
             for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next()) {
-                const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
+                const Unit q = locate(w, begin, tiles, a.groups, unit_rows, kTileC, lane);
                 const int box = q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2, rows = maps.height[box];
                 const CUtensorMap *mx = maps.x + box;
                 const int wrow = (int)(q.e * a.N) + q.n0;
@@ -264,7 +265,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             // even lanes watch the weights' barrier, odd lanes the activations': one round for both
             const bool acts = C::DENSE || (lane & 1);
             for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next(), ti++) {
-                const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
+                const Unit q = locate(w, begin, tiles, a.groups, unit_rows, kTileC, lane);
                 const uint32_t n_mma = (uint32_t)((q.rows + kRowStep - 1) / kRowStep * kRowStep);
                 const int height = maps.height[q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2];
                 const uint32_t b_step = (uint32_t)(height * kOpRow) >> 4;
@@ -326,7 +327,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             uint32_t ph = 1;
             bool ok = true;
             for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next()) {
-                const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
+                const Unit q = locate(w, begin, tiles, a.groups, unit_rows, kTileC, lane);
                 const int wrow = (int)(q.e * a.N) + q.n0;
                 for (int kb = 0; kb < nkb; kb += C::RAWK) {
                     ok = __all_sync(0xffffffffu, ptx::mbar_wait_idle(raw_empty + s, ph, a.status) ? 1 : 0) != 0;
@@ -426,7 +427,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
         bool ok = true;
         int ti = 0;
         for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next(), ti++) {
-            const Unit q = locate(w, begin, tiles, a.groups, BN, kTileC, lane);
+            const Unit q = locate(w, begin, tiles, a.groups, unit_rows, kTileC, lane);
             const int n = q.n0 + quarter * 32 + lane;
             float sc = 1.0f, bi = 0.0f, r = 1.0f;
             if (n < a.N) {
@@ -495,10 +496,12 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     ScaledMaps maps;
     const CUtensorMapDataType xt = C::I8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     const int xe = C::I8 ? 1 : 2;
-    const int last = (int)(a.M % BN + 7) / 8 * 8;         // rows of a plain product's last tile
-    maps.height[1] = a.groups > 1 ? BN / 2 : last ? last : BN;
-    maps.height[2] = a.groups > 1 ? BN / 4 : maps.height[1];
-    maps.height[0] = a.groups == 1 && a.M < BN ? maps.height[1] : BN;        // a plain product without a full tile
+    const int bn = a.unit_rows;
+    const int last = (int)(a.M % bn + 7) / 8 * 8;         // rows of a plain product's last tile
+    maps.height[1] = a.groups > 1 ? bn / 2 : last ? last : bn;
+    maps.height[2] = a.groups > 1 ? bn / 4 : maps.height[1];
+    maps.height[0] = a.groups == 1 && a.M < bn ? maps.height[1] : bn;        // a plain product without a full tile
+    a.row_tiles = (int)((a.M + bn - 1) / bn);
     a.wide = a.K % C::BK == 0;
     const long long w_bytes = a.N * (C::DENSE ? p.ldw : prepack_row_words(a.K, C::I8 ? 1 : 0) * 4);
     // weights that do not stay in L2 between two row tiles (300 x 28672 x 8192 8-bit, 235 MB: 122 -> 82 us; up to 58 MB the two
@@ -522,8 +525,8 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     if (!okw) return TMQ_ERR_LAUNCH;
     int rc = ensure_dynamic_smem(scaled_gemm_kernel<WK, BN>, C::bytes(kMaxGroups));
     if (rc != TMQ_OK) return rc;
-    // at most (rows / BN + groups) row tiles; CTAs beyond the real count find nothing to do
-    const long long units = ((a.M + BN - 1) / BN + a.groups - 1) * ((a.N + kTileC - 1) / kTileC);
+    // at most (rows / bn + groups) row tiles; CTAs beyond the real count find nothing to do
+    const long long units = ((long long)a.row_tiles + a.groups - 1) * ((a.N + kTileC - 1) / kTileC);
     if (units > 0x7FFFFFFF) return TMQ_ERR_UNSUPPORTED;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units < kNumSMs ? units : kNumSMs));
@@ -539,44 +542,64 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
 }
 
 // Rows of a work unit.  Tall tiles use each decoded weight and each copied byte for more rows, low ones leave more units for
-// the SMs and cost less to fill and drain.  Time = base + waves of units * k-blocks * ns per k-block, with what full tiles
-// measured: 155 / 160 / 240 / 352 ns for 32 / 64 / 128 / 256 rows (int8 and bf16 alike within a sixth), 0.6 us more to fill and
-// drain per doubling.  The row tiles of experts are not known here: the even share plus 0.6 of a tile each.  Over 150 shapes
-// (48 .. 2048 rows, 1 .. 128 experts with 1 .. 512 rows each on average) the choice costs 1 % on average against the best
-// tile of each; e.g. 517 x 11008 x 4096 int8 53.0 / 35.3 / 27.8 / 28.5 us, 64 experts (2816 x 2048) of 40 rows 54.0 / 45.2 /
-// 46.6 / 60.8 us, of 512 rows 472 / 275 / 207 / 191 us.
-static int unit_rows(const ScaledArgs &a, int bk) {
+// the SMs and cost less to fill and drain.  Time = base + the first CTA's units * k-blocks * ns per k-block, with what full
+// tiles measured: 155 / 160 / 240 / 352 ns for 32 / 64 / 128 / 256 rows (int8 and bf16 alike within a sixth) and straight
+// lines between 64, 128 and 256, 0.6 us more to fill and drain per doubling.  The row tiles of experts are not known here: the
+// even share plus 0.6 of a tile each.  Over 150 shapes (48 .. 2048 rows, 1 .. 128 experts with 1 .. 512 rows each on average)
+// the choice costs 1 % on average against the best of the four tiles; e.g. 517 x 11008 x 4096 int8 52.9 / 35.6 / 28.3 / 29.0
+// us, 64 experts (2816 x 2048) of 40 rows 54.9 / 45.5 / 47.8 / 61.2 us, of 512 rows 428 / 249 / 200 / 183 us.
+// A plain product's rows are also dealt evenly, in tiles of any multiple of 16 rows, where the waves that whole tiles need
+// leave SMs without work and that promises 4 % (less is lost again to the units' extra operand traffic): the same 517 rows in
+// 24.6 us as three tiles of 176, 1089 x 2253 x 1223 12.1 -> 10.2 us, 4 % on average over 112 random products of 65 .. 4096 rows.
+static int choose_unit_rows(const ScaledArgs &a, int bk) {
     static const double per_block[4] = {0.155, 0.160, 0.240, 0.352};
-    const double blocks = (double)((a.K + bk - 1) / bk), tiles_n = (double)((a.N + kTileC - 1) / kTileC);
+    const long long tiles_n = (a.N + kTileC - 1) / kTileC;
+    const double blocks = (double)((a.K + bk - 1) / bk);
     int best = 32;
-    double best_cost = 0.0;
-    for (int i = 0, bn = 32; i < 4; i++, bn *= 2) {
-        double waves;
-        if (a.groups == 1) {
-            const long long units = (a.M + bn - 1) / bn * ((a.N + kTileC - 1) / kTileC);
-            waves = (double)((units + kNumSMs - 1) / kNumSMs);
-        } else {
-            const double partial = 0.6 * (double)(a.groups < a.M ? a.groups : a.M);
-            waves = ((double)a.M / bn + partial) * tiles_n / kNumSMs;
-            if (waves < 1.0) waves = 1.0;
-        }
-        const double cost = 0.6 * i + waves * blocks * per_block[i];
-        if (i == 0 || cost < best_cost) {
-            best = bn;
+    double best_cost = 1e300;
+    auto consider = [&](int i, int rows, double k_blocks) {
+        const double cost = 0.6 * i + k_blocks * blocks;
+        if (cost < best_cost) {
+            best = rows;
             best_cost = cost;
+        }
+    };
+    for (int i = 0, bn = 32; i < 4; i++, bn *= 2) {
+        if (a.offsets) {
+            const double partial = 0.6 * (double)(a.groups < a.M ? a.groups : a.M);
+            const double waves = ((double)a.M / bn + partial) * (double)tiles_n / kNumSMs;
+            consider(i, bn, (waves < 1.0 ? 1.0 : waves) * per_block[i]);
+            continue;
+        }
+        // k-blocks' time of a unit of `rows` rows, and of the first CTA, which has the most units: `full` of them whole, the rest
+        // of the last row tile
+        auto block = [&](long long rows) {
+            const double below = i > 0 ? per_block[i - 1] : per_block[0];
+            return rows <= bn / 2 ? below : per_block[i] - (per_block[i] - below) * (double)(bn - rows) / (double)(bn / 2);
+        };
+        auto plain = [&](int rows) {
+            const long long tiles = (a.M + rows - 1) / rows, last = a.M - (tiles - 1) * rows;
+            const long long full = ((tiles - 1) * tiles_n + kNumSMs - 1) / kNumSMs, all = (tiles * tiles_n + kNumSMs - 1) / kNumSMs;
+            consider(i, rows, ((double)full * block(rows) + (double)(all - full) * block(last)) * (rows < bn ? 1.04 : 1.0));
+        };
+        plain(bn);
+        if (i >= 2) {
+            const long long waves = ((a.M + bn - 1) / bn * tiles_n + kNumSMs - 1) / kNumSMs, tiles = waves * kNumSMs / tiles_n;
+            const int rows = (int)(((a.M + tiles - 1) / tiles + kRowStep - 1) / kRowStep * kRowStep);
+            if (rows > bn / 2) plain(rows);
         }
     }
     return best;
 }
 
 template <int WK>
-static int dispatch_scaled(const ScaledProblem &p, cudaStream_t st) {
-    switch (unit_rows(p.a, WK == W_TERNARY_BF16 ? 64 : 128)) {
-        case 256: return launch_scaled<WK, 256>(p, st);
-        case 128: return launch_scaled<WK, 128>(p, st);
-        case 64: return launch_scaled<WK, 64>(p, st);
-        default: return launch_scaled<WK, 32>(p, st);
-    }
+static int dispatch_scaled(ScaledProblem p, cudaStream_t st) {
+    const int rows = choose_unit_rows(p.a, WK == W_TERNARY_BF16 ? 64 : 128);
+    p.a.unit_rows = rows;
+    if (rows > 128) return launch_scaled<WK, 256>(p, st);
+    if (rows > 64) return launch_scaled<WK, 128>(p, st);
+    if (rows > 32) return launch_scaled<WK, 64>(p, st);
+    return launch_scaled<WK, 32>(p, st);
 }
 
 static int check_scaled(const ScaledProblem &p, int x_bytes, bool dense) {
@@ -640,7 +663,7 @@ extern "C" int tmq_ternary_gemm_a8(const void *X, int x_type, int64_t ldx, const
         const int rc = launch_token_product(X, x_type, ldx, row_scale, Wt, scale, bias, Y, y_type, M, N, K, ldy, status, st);
         if (rc != TMQ_ERR_UNSUPPORTED) return rc;
     }
-    ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, status}};
+    ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, 0, 0, status}};
     int rc = prepare_a8(p, x_type, false, workspace, workspace_bytes, st);
     if (rc != TMQ_OK || M == 0) return rc;
     if (M <= 8 && x_type >= 0) {         // too many elements to quantise in every CTA, but few rows
@@ -654,7 +677,7 @@ extern "C" int tmq_gemm_i8(const void *X, int x_type, int64_t ldx, const float *
                            const float *scale, const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K,
                            int64_t ldy, void *workspace, size_t workspace_bytes, int *status, void *stream) {
     if (x_type < -1 || x_type > TMQ_TYPE_F16) return TMQ_ERR_ARG;
-    ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, status}};
+    ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, 0, 0, status}};
     const int rc = prepare_a8(p, x_type, true, workspace, workspace_bytes, (cudaStream_t)stream);
     return rc != TMQ_OK || M == 0 ? rc : dispatch_scaled<W_DENSE_I8>(p, (cudaStream_t)stream);
 }
@@ -664,7 +687,7 @@ extern "C" int tmq_ternary_gemm_grouped_bf16(const void *X, int64_t ldx, const u
                                              int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest,
                                              int *status, void *stream) {
     const ScaledProblem p = {X, Wt, ldx, 0,
-                             {nullptr, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, status}};
+                             {nullptr, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 2, false);
     if (rc != TMQ_OK || M == 0) return rc;
@@ -677,7 +700,7 @@ extern "C" int tmq_ternary_gemm_grouped_a8(const int8_t *X, int64_t ldx, const f
                                            int groups, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy,
                                            int zero_rest, int *status, void *stream) {
     const ScaledProblem p = {X, Wt, ldx, 0,
-                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, status}};
+                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 1, false);
     if (rc != TMQ_OK || M == 0) return rc;
@@ -690,7 +713,7 @@ extern "C" int tmq_gemm_grouped_i8(const int8_t *X, int64_t ldx, const float *ro
                                    void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest,
                                    int *status, void *stream) {
     const ScaledProblem p = {X, W, ldx, ldw,
-                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, status}};
+                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 1, true);
     if (rc != TMQ_OK || M == 0) return rc;
