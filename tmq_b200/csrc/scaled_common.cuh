@@ -19,7 +19,6 @@ struct ScaledArgs {
     const void *offsets;             // [groups + 1] int32 or int64, null: one group of all rows
     long long M, N, K, ldy;
     int groups, offsets64, y_type, zero_rest;
-    int wide;                        // K is whole k-blocks: one box per stage
     int unit_rows, row_tiles;        // rows of a work unit, row tiles of a plain product
     int rows_first;                  // order of the work units (plain product only)
     int *status;

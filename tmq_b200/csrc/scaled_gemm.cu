@@ -35,12 +35,15 @@ constexpr int kOpRow = 128;          // bytes of one operand row per k-block: 64
 constexpr int kRowStep = 16;         // granularity of a unit's MMA N
 
 // Tensor maps of a launch.  A TMA instruction costs about 200 cycles of its unit whatever it brings (bf16 tiles of 32 rows
-// with one box per k-block: 154 ns per k-block), so a box spans all k-blocks of a stage where the row length allows it.
+// with one box per k-block: 154 ns per k-block), so a box spans all k-blocks of a stage.  A row that ends inside a k-block has
+// that last stage brought k-block by k-block through maps of the whole row, whose ends are filled with zeros (all stages that
+// way: 32 x 4096 x 4080 ternary 9.7 us against 9.0).
 // Activation boxes come in three heights (multiples of 8: the swizzle's period), a unit takes the lowest that holds its
 // rows.  Rows of a box that lie outside the matrix cost about ten cycles each (one row of 11008 x 4096 8-bit weights: 12.8 us
 // with a box of 32), so a plain product's last tile gets a box of its own height.
 struct ScaledMaps {
-    CUtensorMap x[3], w;
+    CUtensorMap x[3], w;             // boxes of a stage's k-blocks
+    CUtensorMap x_end[3], w_end;     // ... of one
     int height[3];
 };
 
@@ -178,7 +181,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
     int *tiles = begin + a.groups + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int nkb = (int)((a.K + C::BK - 1) / C::BK);
+    const int nkb = (int)((a.K + C::BK - 1) / C::BK), whole = (int)(a.K / C::BK);
     const int tiles_n = (int)((a.N + kTileC - 1) / kTileC);
     const int unit_rows = BN > 64 ? a.unit_rows : BN;        // (low tiles are never balanced)
 
@@ -227,7 +230,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
             for (Walk w(tiles, a, tiles_n); w.more() && ok; w.next()) {
                 const Unit q = locate(w, begin, tiles, a.groups, unit_rows, kTileC, lane);
                 const int box = q.rows > maps.height[1] ? 0 : q.rows > maps.height[2] ? 1 : 2, rows = maps.height[box];
-                const CUtensorMap *mx = maps.x + box;
+                const CUtensorMap *mx = maps.x + box, *mx_end = maps.x_end + box;
                 const int wrow = (int)(q.e * a.N) + q.n0;
                 const uint32_t bytes = (uint32_t)(rows * kOpRow + (C::DENSE ? C::A_BYTES : 0));      // of one k-block
                 for (int kb = 0; kb < nkb; kb += C::KB) {
@@ -236,14 +239,15 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                     if (!ok) break;
                     if (ptx::elect_one()) {
                         uint8_t *wd = smem + C::A_OFF + s * C::KB * C::A_BYTES, *xd = smem + C::B_OFF + s * C::KB * C::B_BYTES;
-                        ptx::mbar_arrive_expect_tx(full + s, bytes * (uint32_t)(a.wide ? C::KB : n));
-                        if (a.wide) {                    // k-blocks beyond the row are filled with zeros, and counted
+                        const bool wide = whole == nkb || kb + C::KB <= whole;
+                        ptx::mbar_arrive_expect_tx(full + s, bytes * (uint32_t)(wide ? C::KB : n));
+                        if (wide) {                      // k-blocks beyond the row are filled with zeros, and counted
                             if (C::DENSE) ptx::tma_load_3d(wd, &maps.w, full + s, 0, wrow, kb);
                             ptx::tma_load_3d(xd, mx, full + s, 0, q.row0, kb);
                         } else {
                             for (int j = 0; j < n; j++) {
-                                if (C::DENSE) ptx::tma_load_3d(wd + j * C::A_BYTES, &maps.w, full + s, (kb + j) * C::BK, wrow, 0);
-                                ptx::tma_load_3d(xd + j * rows * kOpRow, mx, full + s, (kb + j) * C::BK, q.row0, 0);
+                                if (C::DENSE) ptx::tma_load_3d(wd + j * C::A_BYTES, &maps.w_end, full + s, (kb + j) * C::BK, wrow, 0);
+                                ptx::tma_load_3d(xd + j * rows * kOpRow, mx_end, full + s, (kb + j) * C::BK, q.row0, 0);
                             }
                         }
                     }
@@ -502,7 +506,8 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     maps.height[2] = a.groups > 1 ? bn / 4 : maps.height[1];
     maps.height[0] = a.groups == 1 && a.M < bn ? maps.height[1] : bn;        // a plain product without a full tile
     a.row_tiles = (int)((a.M + bn - 1) / bn);
-    a.wide = a.K % C::BK == 0;
+    const long long whole = a.K / C::BK;                  // k-blocks that a row fills
+    const bool wide = whole > 0, ended = a.K % C::BK != 0;
     const long long w_bytes = a.N * (C::DENSE ? p.ldw : prepack_row_words(a.K, C::I8 ? 1 : 0) * 4);
     // weights that do not stay in L2 between two row tiles (300 x 28672 x 8192 8-bit, 235 MB: 122 -> 82 us; up to 58 MB the two
     // orders are within 2 %)
@@ -510,19 +515,29 @@ static int launch_scaled(const ScaledProblem &p, cudaStream_t st) {
     for (int i = 0; i < 3; i++) {        // an encoding costs about half a microsecond: boxes of one height share it
         if (i > 0 && maps.height[i] == maps.height[i - 1]) {
             maps.x[i] = maps.x[i - 1];
+            maps.x_end[i] = maps.x_end[i - 1];
             continue;
         }
-        if (!make_map_blocks(maps.x + i, xt, xe, p.X, (uint64_t)a.K, (uint64_t)a.M, (uint64_t)p.ldx * xe, C::BK, maps.height[i],
-                             C::KB, a.wide))
+        if (wide && !make_map_blocks(maps.x + i, xt, xe, p.X, whole * C::BK, a.M, p.ldx * xe, C::BK, maps.height[i], C::KB, true))
             return TMQ_ERR_LAUNCH;
+        if (ended && !make_map_blocks(maps.x_end + i, xt, xe, p.X, a.K, a.M, p.ldx * xe, C::BK, maps.height[i], 1, false))
+            return TMQ_ERR_LAUNCH;
+        if (!wide) maps.x[i] = maps.x_end[i];
+        if (!ended) maps.x_end[i] = maps.x[i];
     }
     const uint64_t wrows = (uint64_t)a.groups * (uint64_t)a.N;
-    const bool okw = C::DENSE
-        ? make_map_blocks(&maps.w, xt, 1, p.W, (uint64_t)a.K, wrows, (uint64_t)p.ldw, C::BK, kTileC, C::KB, a.wide)
-        : make_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.W, (uint64_t)prepack_valid_words(a.K), wrows,
-                      (uint64_t)prepack_row_words(a.K, C::I8 ? 1 : 0) * 4, C::DENSE ? 4 : C::RAW_PITCH / 4, kTileC,
-                      C::RAW_PITCH == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    bool okw = true;
+    if (C::DENSE) {
+        okw = (!wide || make_map_blocks(&maps.w, xt, 1, p.W, whole * C::BK, wrows, p.ldw, C::BK, kTileC, C::KB, true)) &&
+              (!ended || make_map_blocks(&maps.w_end, xt, 1, p.W, a.K, wrows, p.ldw, C::BK, kTileC, 1, false));
+    } else {
+        okw = make_map_2d(&maps.w, CU_TENSOR_MAP_DATA_TYPE_UINT32, p.W, (uint64_t)prepack_valid_words(a.K), wrows,
+                          (uint64_t)prepack_row_words(a.K, C::I8 ? 1 : 0) * 4, C::DENSE ? 4 : C::RAW_PITCH / 4, kTileC,
+                          C::RAW_PITCH == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+    }
     if (!okw) return TMQ_ERR_LAUNCH;
+    if (C::DENSE && !wide) maps.w = maps.w_end;
+    if (!C::DENSE || !ended) maps.w_end = maps.w;
     int rc = ensure_dynamic_smem(scaled_gemm_kernel<WK, BN>, C::bytes(kMaxGroups));
     if (rc != TMQ_OK) return rc;
     // at most (rows / bn + groups) row tiles; CTAs beyond the real count find nothing to do
@@ -622,8 +637,14 @@ static int check_scaled(const ScaledProblem &p, int x_bytes, bool dense) {
 
 using namespace tmq;
 
-// Scratch of a product whose activations arrive in floating point: their codes (rows of K rounded up to 16), then the scales.
-static long long code_pitch(long long K) { return (K + 15) / 16 * 16; }
+// Scratch of a product whose activations arrive in floating point: their codes, then the scales.  Rows of codes start at
+// multiples of 16 bytes at least, and of up to 128 where that lengthens them by an eighth at most: a copy's 128-byte rows then
+// touch one line instead of two (2048 x 4096 x 4080, both operands: 45.1 us from multiples of 16, 31.8 of 32, 29.6 of 64, 27.1
+// of 128).
+static long long code_pitch(long long K) {
+    const long long unit = K >= 1024 ? 128 : K >= 512 ? 64 : K >= 256 ? 32 : 16;
+    return (K + unit - 1) / unit * unit;
+}
 
 extern "C" size_t tmq_a8_workspace_bytes(int x_type, int64_t M, int64_t K) {
     if (x_type < TMQ_TYPE_F32 || x_type > TMQ_TYPE_F16 || M <= 0 || K <= 0) return 0;
@@ -647,7 +668,7 @@ static int prepare_a8(ScaledProblem &p, int x_type, bool dense, void *workspace,
     if (!workspace || workspace_bytes < tmq_a8_workspace_bytes(x_type, a.M, a.K)) return TMQ_ERR_SCRATCH;
     int8_t *codes = reinterpret_cast<int8_t *>(workspace);
     float *scales = reinterpret_cast<float *>(codes + a.M * q.ldx);
-    rc = tmq_quantize_rows(p.X, x_type, codes, scales, a.M, a.K, p.ldx, q.ldx, q.ldx, st);
+    rc = tmq_quantize_rows(p.X, x_type, codes, scales, a.M, a.K, p.ldx, q.ldx, (a.K + 15) / 16 * 16, st);
     p.X = codes;
     p.ldx = q.ldx;
     a.row_scale = scales;
@@ -663,7 +684,7 @@ extern "C" int tmq_ternary_gemm_a8(const void *X, int x_type, int64_t ldx, const
         const int rc = launch_token_product(X, x_type, ldx, row_scale, Wt, scale, bias, Y, y_type, M, N, K, ldy, status, st);
         if (rc != TMQ_ERR_UNSUPPORTED) return rc;
     }
-    ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, 0, 0, status}};
+    ScaledProblem p = {X, Wt, ldx, 0, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, 0, status}};
     int rc = prepare_a8(p, x_type, false, workspace, workspace_bytes, st);
     if (rc != TMQ_OK || M == 0) return rc;
     if (M <= 8 && x_type >= 0) {         // too many elements to quantise in every CTA, but few rows
@@ -677,7 +698,7 @@ extern "C" int tmq_gemm_i8(const void *X, int x_type, int64_t ldx, const float *
                            const float *scale, const float *bias, void *Y, int y_type, int64_t M, int64_t N, int64_t K,
                            int64_t ldy, void *workspace, size_t workspace_bytes, int *status, void *stream) {
     if (x_type < -1 || x_type > TMQ_TYPE_F16) return TMQ_ERR_ARG;
-    ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, 0, 0, status}};
+    ScaledProblem p = {X, W, ldx, ldw, {row_scale, scale, bias, Y, nullptr, M, N, K, ldy, 1, 0, y_type, 0, 0, 0, 0, status}};
     const int rc = prepare_a8(p, x_type, true, workspace, workspace_bytes, (cudaStream_t)stream);
     return rc != TMQ_OK || M == 0 ? rc : dispatch_scaled<W_DENSE_I8>(p, (cudaStream_t)stream);
 }
@@ -687,7 +708,7 @@ extern "C" int tmq_ternary_gemm_grouped_bf16(const void *X, int64_t ldx, const u
                                              int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest,
                                              int *status, void *stream) {
     const ScaledProblem p = {X, Wt, ldx, 0,
-                             {nullptr, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, 0, status}};
+                             {nullptr, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 2, false);
     if (rc != TMQ_OK || M == 0) return rc;
@@ -700,7 +721,7 @@ extern "C" int tmq_ternary_gemm_grouped_a8(const int8_t *X, int64_t ldx, const f
                                            int groups, void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy,
                                            int zero_rest, int *status, void *stream) {
     const ScaledProblem p = {X, Wt, ldx, 0,
-                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, 0, status}};
+                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 1, false);
     if (rc != TMQ_OK || M == 0) return rc;
@@ -713,7 +734,7 @@ extern "C" int tmq_gemm_grouped_i8(const int8_t *X, int64_t ldx, const float *ro
                                    void *Y, int y_type, int64_t M, int64_t N, int64_t K, int64_t ldy, int zero_rest,
                                    int *status, void *stream) {
     const ScaledProblem p = {X, W, ldx, ldw,
-                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, 0, status}};
+                             {row_scale, scale, bias, Y, offsets, M, N, K, ldy, groups, offsets_bytes == 8, y_type, zero_rest != 0, 0, 0, 0, status}};
     if (offsets_bytes != 4 && offsets_bytes != 8) return TMQ_ERR_ARG;
     const int rc = check_scaled(p, 1, true);
     if (rc != TMQ_OK || M == 0) return rc;
