@@ -19,9 +19,13 @@ struct ScaledArgs {
     const void *offsets;             // [groups + 1] int32 or int64, null: one group of all rows
     long long M, N, K, ldy;
     int groups, offsets64, y_type, zero_rest;
-    int unit_rows, row_tiles;        // rows of a work unit, row tiles of a plain product
-    int rows_first;                  // order of the work units (plain product only)
     int *status;
+    // by the launch:
+    int unit_rows;                   // rows of a work unit
+    int rows_first;                  // order of the work units (plain product only)
+    int minors, majors;              // extents of the order: inner, outer (plain product; experts: the row tiles, on the device)
+    int d_minor, d_major;            // step of a CTA's walk, gridDim.x units
+    int first_mul;                   // x * first_mul >> 16 = x / minors for x < number of SMs
 };
 
 // A product as the C entry points describe it.
@@ -41,27 +45,26 @@ int launch_token_product(const void *X, int x_type, int64_t ldx, const float *ro
 #ifdef __CUDACC__
 // The units of a CTA, every gridDim.x-th.  A whole warp walks; per unit it costs two additions and, for the expert, one look at
 // 32 table entries (a division and a search by one thread took up to 2800 cycles beside busy decode warps, more than the
-// unit's k-blocks).  Channel tiles run fastest, or row tiles (rows_first) where the weights are the larger operand: they are
-// then read from memory once and the activations stay in L2.
+// unit's k-blocks); its divisions are the host's.  Channel tiles run fastest, or row tiles (rows_first) where the weights are
+// the larger operand: they are then read from memory once and the activations stay in L2.
 struct Walk {
     int rt, nt, e;                           // row tile, channel tile, expert
     int d_major, d_minor, minors, majors;
     bool rows_first;
-    // begin[e]: first row of group e, begin[groups]: end of the last; tiles[e]: row tiles before group e
-    __device__ __forceinline__ Walk(const int *tiles, const ScaledArgs &a, int tiles_n) {
+    // tiles[e]: row tiles before group e
+    __device__ __forceinline__ Walk(const int *tiles, const ScaledArgs &a) {
         rows_first = a.rows_first != 0;
-        const int total = tiles[a.groups];
-        minors = rows_first ? total : tiles_n;
-        majors = rows_first ? tiles_n : total;
-        const int first = minors > 0 ? (int)blockIdx.x / minors : 0;
-        d_major = minors > 0 ? (int)gridDim.x / minors : 0;
-        d_minor = (int)gridDim.x - d_major * minors;
+        minors = a.minors;
+        majors = a.offsets ? tiles[a.groups] : a.majors;
+        d_major = a.d_major;
+        d_minor = a.d_minor;
+        const int first = (int)((blockIdx.x * (unsigned)a.first_mul) >> 16);
         const int minor = (int)blockIdx.x - first * minors;
         rt = rows_first ? minor : first;
         nt = rows_first ? first : minor;
         e = 0;
     }
-    __device__ __forceinline__ bool more() const { return minors > 0 && (rows_first ? nt : rt) < majors; }
+    __device__ __forceinline__ bool more() const { return (rows_first ? nt : rt) < majors; }
     __device__ __forceinline__ void next() {
         int &minor = rows_first ? rt : nt, &major = rows_first ? nt : rt;
         major += d_major;
@@ -73,11 +76,23 @@ struct Walk {
     }
 };
 
-// The unit a walk stands on: rows [row0, row0 + rows) of group e, channels [n0, n0 + tile_c).  Whole converged warp.
+// The unit a walk stands on: rows [row0, row0 + rows) of group e, channels [n0, n0 + tile_c).  begin[e]: first row of group e,
+// begin[groups]: end of the last.  Whole converged warp.
 struct Unit {
     int e, row0, rows, n0;
 };
-__device__ __forceinline__ Unit locate(Walk &w, const int *begin, const int *tiles, int groups, int bn, int tile_c, int lane) {
+__device__ __forceinline__ Unit locate(Walk &w, const ScaledArgs &a, const int *begin, const int *tiles, int bn, int tile_c,
+                                       int lane) {
+    const int groups = a.groups;
+    if (!a.offsets) {
+        Unit q;
+        q.e = 0;
+        q.n0 = w.nt * tile_c;
+        q.row0 = w.rt * bn;
+        const int left = (int)a.M - q.row0;
+        q.rows = left < bn ? left : bn;
+        return q;
+    }
     for (;;) {                               // tiles[] does not decrease: the entries at or below rt are a prefix
         const int i = w.e + 1 + lane;
         const int n = __popc(__ballot_sync(0xffffffffu, i <= groups && tiles[i] <= w.rt));
@@ -95,13 +110,6 @@ __device__ __forceinline__ Unit locate(Walk &w, const int *begin, const int *til
 
 // Executed by one warp: boundaries -> table.  Chunks of 32 boundaries, a running maximum and a running sum of tiles.
 __device__ __forceinline__ void build_table(const ScaledArgs &a, int *begin, int *tiles, int bn, int lane) {
-    if (!a.offsets) {
-        if (lane == 0) {
-            begin[0] = 0; begin[1] = (int)a.M;
-            tiles[0] = 0; tiles[1] = a.row_tiles;
-        }
-        return;
-    }
     int run = 0, sum = 0;                                       // running maximum of the boundaries, tiles so far
     for (int c = 0; c <= a.groups; c += 32) {
         const int i = c + lane;
