@@ -102,59 +102,72 @@ struct ScaledCfg {
     static_assert(TAB_OFF + 2 * 4 * (kMaxGroups + 1) + 1024 <= 227 * 1024, "shared memory exceeded");
 };
 
-// One warp's COUNT rows x 32 channels (f[j]: row j of this lane's channel) to Y.  TYPE fixed at compile time, addresses
-// stepped.  FULL: all of them exist.  PAIRS: 16-bit results of two rows are paired between neighbouring lanes (even lanes keep
-// row j, odd lanes row j + 1), so a warp writes 4 bytes a lane, two 64-byte runs; otherwise one row's 32 channels at a time.
-template <int TYPE, bool PAIRS, bool FULL, int COUNT>
-__device__ __forceinline__ void store_rows(uint8_t *Y, long long row, long long ldy, int n, long long N, int left, int lane,
-                                           const float (&f)[COUNT]) {
+// COUNT accumulator columns (rows of the result) of this lane's channel, scaled and rounded, to Y.  rs: their row scales (16-byte
+// aligned).  TYPE fixed at compile time, addresses stepped.  FULL: all rows and channels exist.  PAIRS: two rows' 16-bit results
+// make a word, and neighbouring lanes exchange halves (even lanes keep row j, odd lanes row j + 1), so a warp writes 4 bytes a
+// lane, two 64-byte runs; otherwise one row's 32 channels at a time.  One warp per scheduler does this and is bound by its own
+// instructions, 19 cycles a row; each step is made for all rows before the next, so that their latencies overlap (four rows at
+// a time: 33 cycles a row; conversions by an addition of 1.5 * 2^23, or no stores at all, changed nothing).
+template <bool I8, int TYPE, bool PAIRS, bool FULL, int COUNT>
+__device__ __forceinline__ void store_rows(const uint32_t (&v)[COUNT], const float *rs, float sc, float bi, uint8_t *Y, long long row,
+                                           long long ldy, int n, long long N, int left, int lane) {
     constexpr int ES = TYPE == TMQ_TYPE_F32 ? 4 : 2;
     const int odd = PAIRS ? lane & 1 : 0;
+    const uint32_t pick = odd ? 0x3276u : 0x5410u;
     const int nb = n - odd;
     uint8_t *p = Y + ((row + odd) * ldy + nb) * ES;
     const long long step = ldy * ES;
     const int rows = nb < N ? left - odd : 0;
     const bool both = nb + 1 < N;
+    float f[COUNT];
 #pragma unroll
-    for (int j = 0; j < COUNT; j += (PAIRS ? 2 : 1)) {
-        if (PAIRS) {
-            const float got = __shfl_xor_sync(0xffffffffu, odd ? f[j] : f[j + (PAIRS ? 1 : 0)], 1);
-            const float lo = odd ? got : f[j], hi = odd ? f[j + (PAIRS ? 1 : 0)] : got;
-            uint32_t w;
+    for (int j = 0; j < COUNT; j += 4) {
+        float4 r = make_float4(1.0f, 1.0f, 1.0f, 1.0f);
+        if (I8) r = *reinterpret_cast<const float4 *>(rs + j);
+        const float rj[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            f[j + i] = fmaf(I8 ? __fmul_rn(__int2float_rn((int)v[j + i]), rj[i]) : __uint_as_float(v[j + i]), sc, bi);
+    }
+    if (PAIRS) {
+        uint32_t w[COUNT / 2];
+#pragma unroll
+        for (int j = 0; j < COUNT / 2; j++) {
             if (TYPE == TMQ_TYPE_BF16) {
-                const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-                w = *reinterpret_cast<const uint32_t *>(&h);
+                const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t *>(&h);
             } else {
-                const __half2 h = __floats2half2_rn(lo, hi);
-                w = *reinterpret_cast<const uint32_t *>(&h);
+                const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t *>(&h);
             }
-            if (FULL || j < rows) {
-                if (FULL || both) *reinterpret_cast<uint32_t *>(p) = w;
-                else *reinterpret_cast<uint16_t *>(p) = (uint16_t)w;
+        }
+#pragma unroll
+        for (int j = 0; j < COUNT / 2; j++) w[j] = __byte_perm(w[j], __shfl_xor_sync(0xffffffffu, w[j], 1), pick);
+#pragma unroll
+        for (int j = 0; j < COUNT / 2; j++) {
+            if (FULL || 2 * j < rows) {
+                if (FULL || both) *reinterpret_cast<uint32_t *>(p) = w[j];
+                else *reinterpret_cast<uint16_t *>(p) = (uint16_t)w[j];
             }
             p += 2 * step;
-        } else {
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < COUNT; j++) {
             if (FULL || j < rows) store_one(p, TYPE, 0, f[j]);
             p += step;
         }
     }
 }
 
-// COUNT accumulator columns (rows of the result) of this lane's channel -> results.  rs: their row scales, or null for 1.
 template <bool I8, int COUNT>
 __device__ __forceinline__ void finish_rows(const uint32_t (&v)[COUNT], const float *rs, float sc, float bi, const ScaledArgs &a,
                                             bool pairs, long long row, int n, int left, int lane) {
-    float f[COUNT];
-#pragma unroll
-    for (int j = 0; j < COUNT; j++) {
-        const float acc = I8 ? __fmul_rn(__int2float_rn((int)v[j]), rs[j]) : __uint_as_float(v[j]);
-        f[j] = fmaf(acc, sc, bi);
-    }
     uint8_t *Y = reinterpret_cast<uint8_t *>(a.Y);
     const bool full = left >= COUNT && n - lane + 32 <= a.N;
 #define TMQ_STORE(TYPE, PAIRS)                                                                            \
-    (full ? store_rows<TYPE, PAIRS, true, COUNT>(Y, row, a.ldy, n, a.N, left, lane, f)                    \
-          : store_rows<TYPE, PAIRS, false, COUNT>(Y, row, a.ldy, n, a.N, left, lane, f))
+    (full ? store_rows<I8, TYPE, PAIRS, true, COUNT>(v, rs, sc, bi, Y, row, a.ldy, n, a.N, left, lane)    \
+          : store_rows<I8, TYPE, PAIRS, false, COUNT>(v, rs, sc, bi, Y, row, a.ldy, n, a.N, left, lane))
     if (a.y_type == TMQ_TYPE_F32) TMQ_STORE(TMQ_TYPE_F32, false);
     else if (a.y_type == TMQ_TYPE_BF16) pairs ? TMQ_STORE(TMQ_TYPE_BF16, true) : TMQ_STORE(TMQ_TYPE_BF16, false);
     else pairs ? TMQ_STORE(TMQ_TYPE_F16, true) : TMQ_STORE(TMQ_TYPE_F16, false);
