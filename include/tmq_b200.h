@@ -250,10 +250,10 @@ int tmq_ternary_gemv_batched_i8(const int8_t *X, int64_t x_stride, const uint32_
  *
  * tmq_quantize_rows: X [M][ldx] (TMQ_TYPE_*) -> codes Q int8 [M][ldq] and one scale per row:
  *   amax = max_k |x_k|,  scale = amax / 127 (one fp32 rounding),  q_k = round-half-even(127 x_k / amax), decided exactly.
- * Columns K .. cols - 1 of Q are set to zero (K <= cols <= ldq), the rest of a row is left alone.  amax = 0: scale 0, codes 0.  A NaN or an infinity in a row: scale NaN, codes 0
- * (the products of that row are NaN, other rows are unaffected).  Rows of a weight matrix quantise the same way (one scale
- * per output channel).  Any M, K, alignment; 16-byte aligned rows of X and Q with ldq % 16 == 0 and cols % 16 == 0 take the
- * vector accesses.
+ * Columns K .. cols - 1 of Q are set to zero (K <= cols <= ldq), the rest of a row is left alone.  amax = 0: scale 0, codes
+ * 0.  A NaN or an infinity in a row: scale NaN, codes 0 (the products of that row are NaN, other rows are unaffected).  Rows
+ * of a weight matrix quantise the same way (one scale per output channel).  Any M, K, alignment; 16-byte aligned rows of X
+ * and Q with ldq % 16 == 0 and cols % 16 == 0 take the vector accesses.
  * extends: Linear.compact_forward, tmq/tmq.py:662-688 (fp32 activations only).
  * ------------------------------------------------------------------------------------------------ */
 #define TMQ_TYPE_F32 0
@@ -272,8 +272,12 @@ int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *scale, int64_
  *   (TMQ_ERR_SCRATCH without it, before anything is launched).  tmq_ternary_gemm_a8 needs none for M <= 8 and
  *   M K <= TMQ_A8_FUSED_ELEMS where an SM's share of the matrix fits its shared memory (N <= 11840 and rows of a few
  *   thousand): quantisation and product are then one launch.
- * Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw], 16-byte aligned, ldw % 16 == 0.
- * Y [M][ldy], element-aligned.  *status: see "Status word" above.
+ * Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw], 16-byte aligned, ldw % 16 == 0.  Rows of 8-bit
+ * operands that start at multiples of 128 bytes are read up to 1.6 times as fast as rows at odd multiples of 16.
+ * Y [M][ldy], element-aligned, apart from the operands.  *status: see "Status word" above.
+ * These launches, and tmq_quantize_rows, let the next launch of the stream start early.  They read all operands after their
+ * predecessor's end; the skinny kernels above fetch scale and bias ahead of it, so a result of one of these launches must not
+ * be the scale or bias of a skinny launch right behind it.
  * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549, ternary_mvm_cuda, :563-603, and the post_scale / bias of
  * Linear.compact_forward, tmq/tmq.py:662-688 (fp32 activations on CUDA cores). */
 #define TMQ_A8_FUSED_ELEMS 16384

@@ -906,7 +906,7 @@ def ternary_gemm_a8(x, wt, columns, row_scale=None, scale=None, bias=None, out_d
     x: CUDA int8 [M, K] (any row stride; row_scale fp32 [M] or None for 1), or fp32 / bf16 / fp16 [M, K], which is quantised
     here exactly as quantize_rows does (inside the product's launch for a few rows).  wt: prepack(..., FMT_I8) (its rows are
     padded, so a width close to the weights' own is not told apart from it).  scale, bias: fp32 [columns] or None.  out:
-    optional [M, columns] tensor of the output dtype whose rows may be strided.  No gradient."""
+    optional [M, columns] tensor of the output dtype whose rows may be strided, apart from the operands.  No gradient."""
     name = "ternary_gemm_a8"
     code, M, K, dev = _rows_in(name, x, _A8_TYPES)
     N = int(columns)
