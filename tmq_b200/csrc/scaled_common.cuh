@@ -8,10 +8,6 @@
 
 namespace tmq {
 
-enum { W_TERNARY_BF16 = 0, W_TERNARY_I8 = 1, W_DENSE_I8 = 2 };
-
-constexpr int kMaxGroups = TMQ_GROUPS_MAX;
-
 struct ScaledArgs {
     const float *row_scale;          // [M] or null (1)
     const float *scale, *bias;       // [groups][N] or null (1 / 0)
