@@ -124,6 +124,14 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, i
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, status, budget) ? 1 : 0) != 0;
 }
 
+// A vote of a converged warp whose lanes have watched different barriers.  The vote itself orders no memory: the
+// synchronisation behind it passes on to every lane what the others saw complete.
+__device__ __forceinline__ bool all_lanes(bool mine) {
+    const bool all = __all_sync(0xffffffffu, mine ? 1 : 0) != 0;
+    __syncwarp();
+    return all;
+}
+
 // The whole-warp wait and the arrival on shared-window addresses, for loops whose barrier addresses are stepped rather than
 // indexed: a decode warp's round is short enough that pointer arithmetic shows.
 __device__ __forceinline__ bool mbar_wait_warp_at(uint32_t bar, uint32_t parity, int *status,
@@ -150,7 +158,7 @@ __device__ __forceinline__ bool mbar_wait_warp_at(uint32_t bar, uint32_t parity,
             if (!ok) break;
         }
     }
-    return __all_sync(0xffffffffu, ok ? 1 : 0) != 0;
+    return all_lanes(ok);
 }
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");

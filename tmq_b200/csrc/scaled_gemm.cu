@@ -244,7 +244,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                 ptx::tc_fence_after_sync();
                 const uint32_t d_tmem = tmem_base + (uint32_t)(buf * BN);
                 for (int kb = 0; kb < nkb; kb += C::KB) {
-                    if (!landed) ok = ptx::mbar_wait_warp(acts ? full + sb : ready + sa, acts ? pb : pa, a.status);
+                    if (!landed) ok = ptx::all_lanes(ptx::mbar_wait(acts ? full + sb : ready + sa, acts ? pb : pa, a.status));
                     if (!ok) break;
                     ptx::tc_fence_after_sync();
                     const uint64_t a_desc = ptx::umma_desc_sw128(ptx::smem_u32(smem + C::A_OFF + sb * C::KB * C::A_BYTES));
@@ -275,7 +275,7 @@ scaled_gemm_kernel(const __grid_constant__ ScaledMaps maps, const ScaledArgs a) 
                         ptx::umma_commit(used_b);
                         if (!C::DENSE) ptx::umma_commit(used_a);
                     }
-                    landed = __all_sync(0xffffffffu, next ? 1 : 0) != 0;
+                    landed = ptx::all_lanes(next);
                 }
                 if (ok && ptx::elect_one()) ptx::umma_commit(acc_full + buf);
                 __syncwarp();
