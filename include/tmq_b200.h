@@ -217,10 +217,10 @@ int tmq_ternary_gemm_bf16_bcast(const void *X, const uint32_t *Wt, const float *
  * launch), so consecutive launches overlap their weight traffic with the predecessor's arithmetic; `status` (device
  * int, zero before the first call, may be NULL: then the non-resident streaming kernel is used) receives
  * TMQ_ERR_TIMEOUT if those copies never complete.
- * CONTRACT that follows from the early fetch: Wt, scale and bias must be complete in memory before the kernel that
- * PRECEDES this call in the stream starts, i.e. they must not be written by the immediately preceding launch
- * (tmq_prepack ends with an empty kernel for exactly this reason; weights written by a caller's own kernel need one
- * launch or an event between them and this call).  X and Y carry no such restriction.
+ * CONTRACT that follows from the early fetch: Wt must be complete in memory before the kernel that PRECEDES this call in
+ * the stream starts, i.e. it must not be written by the immediately preceding launch (tmq_prepack ends with an empty
+ * kernel for exactly this reason; weights written by a caller's own kernel need one launch or an event between them and
+ * this call).  X, scale, bias and Y carry no such restriction.
  * replaces: ternary_mvm_cuda, tmq/tmq_cuda.cu:563-603 (kernel :242-286). */
 int tmq_ternary_gemv_bf16(const void *X, const uint32_t *Wt, const float *scale, const float *bias, void *Y, int64_t M,
                           int64_t N, int64_t K, int64_t ldy, int out_f32, int *status, void *stream);
@@ -275,9 +275,8 @@ int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *scale, int64_
  * Wt: tmq_prepack fmt 1 of the packed ternary weights, or W int8 [N][ldw], 16-byte aligned, ldw % 16 == 0.  Rows of 8-bit
  * operands that start at multiples of 128 bytes are read up to 1.6 times as fast as rows at odd multiples of 16.
  * Y [M][ldy], element-aligned, apart from the operands.  *status: see "Status word" above.
- * These launches, and tmq_quantize_rows, let the next launch of the stream start early.  They read all operands after their
- * predecessor's end; the skinny kernels above fetch scale and bias ahead of it, so a result of one of these launches must not
- * be the scale or bias of a skinny launch right behind it.
+ * These launches, and tmq_quantize_rows, let the next launch of the stream start early and read all operands after their
+ * predecessor's end.
  * extends: ternary_mmm_cuda, tmq/tmq_cuda.cu:478-549, ternary_mvm_cuda, :563-603, and the post_scale / bias of
  * Linear.compact_forward, tmq/tmq.py:662-688 (fp32 activations on CUDA cores). */
 #define TMQ_A8_FUSED_ELEMS 16384

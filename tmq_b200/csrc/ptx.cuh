@@ -205,6 +205,12 @@ __device__ __forceinline__ void prefetch_l2(const void *gsrc, uint32_t bytes) {
     asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(reinterpret_cast<uint64_t>(gsrc)), "r"(bytes) : "memory");
 }
 
+// One 32-bit word global -> shared, and the wait of a thread for all such copies of its own
+__device__ __forceinline__ void copy_async4(void *smem_dst, const void *gsrc) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(smem_dst)), "l"(gsrc) : "memory");
+}
+__device__ __forceinline__ void copy_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 // 256-bit global accesses (32-byte aligned): a lane moves a whole 32-byte sector with one request.  An epilogue whose
 // threads each own an output row otherwise writes every sector with two 16-byte requests from two instructions.
 struct u32x8 {

@@ -12,8 +12,8 @@
 //
 // Common to both:
 //   * consecutive launches are chained with programmatic dependent launch: weights depend on nothing, so they are
-//     requested while the previous launch is still computing; activations and outputs are only touched after
-//     griddepcontrol.wait, i.e. after the previous kernel in the stream has completed.
+//     requested while the previous launch is still computing; everything else (activations, scale, bias, outputs) is only
+//     touched after griddepcontrol.wait, i.e. after the previous kernel in the stream has completed.
 //   * arithmetic: a 2-bit code costs about one integer instruction to decode, which already fills half the issue
 //     slots at HBM speed; an fp32 add/sub per weight on top (the CUDA-core formulation) cannot keep up.  The decoded
 //     codes are fed, exact, to warp-level mma (m16n8k16 bf16 / m16n8k32 s8) with the <= 8 activation rows as the 8
@@ -551,23 +551,7 @@ __global__ void __launch_bounds__(WARPS * 32, 2) ternary_gemv_resident_kernel(co
     int group0, G;
     resident_groups(a, group0, G);
     resident_prologue(a, wsm, bar, group0, G);
-    // per-channel scale / bias of the outputs this thread will write (they belong to the weights, not to the chain):
-    // fetched here so that their latency is not paid after the arithmetic
-    float psc[ResOut<WARPS>::passes], pbi[ResOut<WARPS>::passes];
-    if (KIND == 0) {
-#pragma unroll
-        for (int q = 0; q < ResOut<WARPS>::passes; q++) {
-            psc[q] = 0.5f;                                    // operands carried +-2.0
-            pbi[q] = 0.0f;
-            const int o = threadIdx.x + q * (WARPS * 32);
-            const long long n = ((long long)group0 + (o >> 7)) * 16 + (o & 15);
-            if (o < G * 128 && n < a.N) {
-                if (a.scale) psc[q] *= a.scale[n];
-                if (a.bias) pbi[q] = a.bias[n];
-            }
-        }
-    }
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // activations and outputs belong to the chain
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // all but the packed rows may come from the chain
     __syncthreads();                                     // the barrier warp 0 initialised is visible to every warp
 
     Acc acc[kResGroups][4];
@@ -577,8 +561,17 @@ __global__ void __launch_bounds__(WARPS * 32, 2) ternary_gemv_resident_kernel(co
         for (int j = 0; j < 4; j++) acc[i][j] = 0;
     uint32_t xr[R::XR];
     R::load_x(a.X, a.M, a.K, warp, g, t, xr);      // in flight while the last packed rows land
+    // Scale and bias of this CTA's channels travel into shared memory under the arithmetic.  Behind the wait: a launch before this
+    // one may have written them and released this one early.  (Held in registers from here on: 4.9 us instead of 4.2 for 8 rows of
+    // 4096 x 4096.)
+    __shared__ float coeff[2][kResGroups * 16];
+    if (KIND == 0 && threadIdx.x < G * 16 && (long long)group0 * 16 + threadIdx.x < a.N) {
+        if (a.scale) ptx::copy_async4(&coeff[0][threadIdx.x], a.scale + (long long)group0 * 16 + threadIdx.x);
+        if (a.bias) ptx::copy_async4(&coeff[1][threadIdx.x], a.bias + (long long)group0 * 16 + threadIdx.x);
+    }
     const bool ok = __syncthreads_and(ptx::mbar_wait(bar, 0, a.status));
     if (ok) R::template slices<FULL>(wsm, a.X, a.M, a.K, a.KS, G, warp, g, t, xr, acc);
+    if (KIND == 0) ptx::copy_async_wait();
     __syncthreads();   // every warp is done reading the packed rows: the area becomes the reduction buffer
     if (!ok) return;   // uniform: the copies never completed and the status word says so
     Acc *red = reinterpret_cast<Acc *>(wsm);  // [warp][group][16][8]
@@ -595,7 +588,8 @@ __global__ void __launch_bounds__(WARPS * 32, 2) ternary_gemv_resident_kernel(co
             if (KIND == 1) {
                 reinterpret_cast<int *>(a.Y)[(long long)col * a.ldy + n] = (int)s;
             } else {
-                const float f = fmaf((float)s, psc[q], pbi[q]);
+                const float sc = (a.scale ? coeff[0][grp * 16 + row] : 1.0f) * 0.5f;   // operands carried +-2.0
+                const float f = fmaf((float)s, sc, a.bias ? coeff[1][grp * 16 + row] : 0.0f);
                 if (a.out_f32) reinterpret_cast<float *>(a.Y)[(long long)col * a.ldy + n] = f;
                 else reinterpret_cast<__nv_bfloat16 *>(a.Y)[(long long)col * a.ldy + n] = __float2bfloat16_rn(f);
             }
