@@ -461,30 +461,45 @@ class _StatusWatch:
     launch skip its work (the word is sticky) while the C calls keep returning TMQ_OK, so somebody has to look: every
     `EVERY` launches the word is copied to pinned host memory behind the work already queued, and the next operator
     call that finds the copy finished raises if it is non-zero.  No synchronisation is added; a failure surfaces
-    within about 2 * EVERY operator calls instead of never."""
+    within about 2 * EVERY operator calls instead of never.  A call that is being captured starts no copy (it would
+    become part of the graph) and raises nothing; what falls due there is done by the next call outside a capture."""
 
     EVERY = 32
-    POLL = 8         # launches between two looks: an event query alone costs 1.5 us of host time
+    UNREAD = 0x7FFFFFFF      # what the host's word holds until a copy has landed; no kernel stores it
 
     def __init__(self, device):
         self.device = device
         self.host = torch.zeros(1, dtype=torch.int32).pin_memory()
-        self.event = torch.cuda.Event()
+        # the host's word, looked at without a call into CUDA: an event query costs 1.5 us and would invalidate a capture
+        self.word = ctypes.c_int32.from_address(self.host.data_ptr())
         self.pending = False
         self.launches = 0
+        self.due = 1             # launch from which on the next copy is made
+
+    def capturing(self):
+        if torch.cuda.is_current_stream_capturing():
+            return True
+        if torch.cuda.current_device() == self.device.index:
+            return False
+        with torch.cuda.device(self.device):
+            return torch.cuda.is_current_stream_capturing()
 
     def note_launch(self):
         self.launches += 1
-        if self.launches % self.POLL != 1 or torch.cuda.is_current_stream_capturing():
-            return                                # (a query would invalidate a capture, a copy would become part of it)
-        if self.pending and self.event.query():
-            self.pending = False
-            code = int(self.host[0])
+        if self.pending:
+            code = self.word.value
+            if code == self.UNREAD:
+                return
             if code != 0:
+                if self.capturing():
+                    return
+                self.pending = False
                 _raise_status(self.device, code)
-        if not self.pending and self.launches % self.EVERY == 1:
+            self.pending = False
+        if self.launches >= self.due and not self.capturing():
+            self.due = self.launches + self.EVERY
+            self.word.value = self.UNREAD
             self.host.copy_(gemm_status_word(self.device), non_blocking=True)
-            self.event.record()
             self.pending = True
 
 
