@@ -637,7 +637,14 @@ class PackedExperts(nn.Module):
     layers: compact Linear layers (compressed_state_dict, load_compressed_state_dict) with equal shapes, on one GPU, without
     an implicit batch norm.  Their weights are copied into one stack, their post_scale and bias into one table each; later
     changes of the layers do not show.  activation_bits: None multiplies bf16 rows as they are (fp32 accumulation), 8
-    quantises each row (fp32, bf16 or fp16) to 8 bits with a scale of its own."""
+    quantises each row (fp32, bf16 or fp16) to 8 bits with a scale of its own.
+
+    The stack, the tables and activation_bits are part of the state dict; loading one restores all three for a module of the
+    same widths and number of experts, whatever layers it was made from.  Casts of the module (half, to(dtype)) leave the
+    tables in fp32."""
+
+    _version = 2             # 1: the stack was not part of the state dict
+    _TABLES = ("scales", "biases")
 
     def __init__(self, layers, activation_bits=None):
         super().__init__()
@@ -663,14 +670,53 @@ class PackedExperts(nn.Module):
             weights = torch.stack([ops.prepack(layer._packed_matrix(), self.out_features, fmt) for layer in layers])
             scales = biases = None
             if any(layer.post_scale_imm != 1.0 for layer in layers):
-                scales = torch.tensor([float(layer.post_scale_imm) for layer in layers], device=dev)
+                scales = torch.tensor([float(layer.post_scale_imm) for layer in layers], dtype=torch.float32, device=dev)
                 scales = scales[:, None].expand(len(layers), self.out_features).contiguous()
             if any(layer.bias is not None for layer in layers):
-                zero = torch.zeros(self.out_features, device=dev)
+                zero = torch.zeros(self.out_features, dtype=torch.float32, device=dev)
                 biases = torch.stack([zero if layer.bias is None else layer.bias.detach().float().to(dev) for layer in layers])
-        self.register_buffer("weights", weights, persistent=False)
-        self.register_buffer("scales", scales, persistent=False)
-        self.register_buffer("biases", biases, persistent=False)
+        self.register_buffer("weights", weights)
+        self.register_buffer("scales", scales)
+        self.register_buffer("biases", biases)
+
+    def _apply(self, fn, recurse=True):
+        tables = {name: getattr(self, name) for name in self._TABLES}
+        super()._apply(fn, recurse)
+        for name, table in tables.items():
+            if table is not None and getattr(self, name).dtype != torch.float32:
+                setattr(self, name, table.to(getattr(self, name).device))
+        return self
+
+    def get_extra_state(self):
+        return torch.tensor([self.activation_bits or 0, self.out_features, self.in_features])
+
+    def set_extra_state(self, state):
+        self.activation_bits = int(state[0]) or None
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
+        held = {name: state_dict.get(prefix + name) for name in ("weights",) + self._TABLES}
+        if local_metadata.get("version") == 1 and all(t is None for t in held.values()):
+            return                                        # written before the stack was saved: what the layers gave stays
+        extra = state_dict.get(prefix + "_extra_state")
+        if held["weights"] is not None:
+            # words of other widths can fill rows of the same length, so the widths are compared themselves
+            shape = None
+            if extra is not None and [int(v) for v in extra[1:]] == [self.out_features, self.in_features]:
+                fmt = ops.FMT_I8 if int(extra[0]) == 8 else ops.FMT_BF16
+                shape = (self.weights.shape[0], self.out_features, ops.prepack_row_words(self.in_features, fmt))
+            if shape is None or tuple(held["weights"].shape) != shape:
+                error_msgs.append(f"{prefix[:-1]}: the saved experts are not {self!r}")
+                return
+            if tuple(self.weights.shape) != shape:        # saved with the other activation_bits
+                self.weights = torch.empty(shape, dtype=torch.int32, device=self.weights.device)
+            for name in self._TABLES:                     # a table is there or not as it was saved
+                if held[name] is None:
+                    setattr(self, name, None)
+                elif getattr(self, name) is None:
+                    setattr(self, name, torch.empty((self.weights.shape[0], self.out_features), dtype=torch.float32,
+                                                    device=self.weights.device))
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys, error_msgs)
 
     def __repr__(self):
         return "PackedExperts(%d x %d,%d) [tmq]" % (self.weights.shape[0], self.out_features, self.in_features)
