@@ -6,7 +6,8 @@ What is kept (reference file:line in brackets): `QuantMode`, `TensorType` [tmq/t
 [:315-438] and `SoftStepDerivative` [:441-493], the layer drop-ins `Linear` [:573-765], `Conv2d` [:769-973],
 `ConvTranspose2d` [:978-1087], and the model-level helpers `quantize_weights`, `quantize_model`,
 `compressed_state_dict`, `prepare_compressed_load`, `load_compressed_state_dict`, `expand_compact_layers`
-[:1090-1319], including the state-dict metadata keys `tmq.tensor_type`, `tmq.shape`, `tmq.quant`.
+[:1090-1319], including the state-dict metadata keys `tmq.tensor_type`, `tmq.shape`, `tmq.quant` (`tmq.activation_bits`, where set, is
+this package's own).
 
 What differs, on purpose:
   * the soft-step functions, the quantization loss, the clamp, packing and compact inference run in the CUDA
@@ -527,6 +528,8 @@ class TMQLayer:
             else:
                 self.compact = False
             self.quantization = QuantMode(local_metadata["tmq.quant"])
+            if "tmq.activation_bits" in local_metadata:
+                self.activation_bits = local_metadata["tmq.activation_bits"]
             self.training = False if self.compact else self.training
         else:
             self.compact = False
@@ -1022,7 +1025,8 @@ def _tmq_layers(module, prefix=""):
 def set_activation_bits(module: nn.Module, bits):
     """Precision of the activations in the compact (packed) inference of every TMQ Linear layer of `module`: 8 quantises each
     row to 8 bits with a scale of its own (ops.ternary_gemm_a8), None multiplies the activations as they come.  Training and
-    uncompressed layers are not affected.  No counterpart in the reference."""
+    uncompressed layers are not affected.  compressed_state_dict saves the setting, load_compressed_state_dict restores it; a
+    state dict without one leaves the layer's.  No counterpart in the reference."""
     if bits not in (None, 8):
         raise ValueError("set_activation_bits: bits must be None or 8")
     for sub in module.modules():
@@ -1095,6 +1099,8 @@ def compressed_state_dict(module: nn.Module, strong=False, remove_prefix=""):
         meta["tmq.tensor_type"] = layer.tensor_type.value
         meta["tmq.shape"] = layer.original_shape
         meta["tmq.quant"] = layer.quantization.value
+        if getattr(layer, "activation_bits", None) is not None:
+            meta["tmq.activation_bits"] = layer.activation_bits
         if layer.tensor_type == TensorType.COMPRESSED_TERNARY_32BIT:
             # keep the live model usable: back to the packed form (on the device the layer lived on)
             packed = decompress_ternary(layer.weight.data, layer.original_shape)
