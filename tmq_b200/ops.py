@@ -772,9 +772,14 @@ _status_address = {}
 
 # The calls below are a few microseconds long for single tokens, and their host side is kept to as little: one pass over the
 # arguments, torch.empty_strided (torch.empty with a shape tuple costs a microsecond more), raw streams, no device context for
-# the device that is current anyway.
-_current_device = getattr(torch._C, "_cuda_getDevice", None)
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+# the device that is current anyway.  The two functions taken from torch._C are not part of torch's interface: where they
+# are missing, the public ones do the same a little more slowly.
+def _public_raw_stream(index):
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or _public_raw_stream
 
 
 def _status_word_address(index):
