@@ -252,8 +252,8 @@ int tmq_ternary_gemv_batched_i8(const int8_t *X, int64_t x_stride, const uint32_
  *   amax = max_k |x_k|,  scale = amax / 127 (one fp32 rounding),  q_k = round-half-even(127 x_k / amax), decided exactly.
  * Columns K .. cols - 1 of Q are set to zero (K <= cols <= ldq), the rest of a row is left alone.  amax = 0: scale 0, codes
  * 0.  A NaN or an infinity in a row: scale NaN, codes 0 (the products of that row are NaN, other rows are unaffected).  Rows
- * of a weight matrix quantise the same way (one scale per output channel).  Any M, K, alignment; 16-byte aligned rows of X
- * and Q with ldq % 16 == 0 and cols % 16 == 0 take the vector accesses.
+ * of a weight matrix quantise the same way (one scale per output channel).  Any M, K, alignment; vector loads are taken for
+ * rows of X that start at multiples of 16 bytes, vector stores where Q, ldq and cols are multiples of 8 (4 for fp32 X).
  * extends: Linear.compact_forward, tmq/tmq.py:662-688 (fp32 activations only).
  * ------------------------------------------------------------------------------------------------ */
 #define TMQ_TYPE_F32 0
@@ -263,7 +263,7 @@ int tmq_quantize_rows(const void *X, int x_type, int8_t *Q, float *scale, int64_
                       int64_t cols, void *stream);
 
 /* Y[m][n] = acc * row_scale[m] * scale[n] + bias[n],  acc = sum_k q[m][k] W[n][k] exact in int32 (K <= 131071), then fp32:
- * (acc * row_scale) rounded, times scale plus bias in one fused multiply-add, rounded once more to y_type (TMQ_TYPE_*).
+ * acc rounded, (acc * row_scale) rounded, times scale plus bias in one fused multiply-add, rounded once more to y_type (TMQ_TYPE_*).
  * scale [N], bias [N]: fp32, NULL for 1 / 0.
  * x_type -1: X holds the codes, int8 [M][ldx], 16-byte aligned, ldx % 16 == 0, any K <= ldx (columns beyond K are not used),
  *   row_scale fp32 [M] or NULL for 1.

@@ -15,9 +15,10 @@
 //   * Every wait is bounded (TMQ_ERR_TIMEOUT in the status word).
 //
 // What bounds it: tall tiles the tensor pipe (bf16 256 rows: the 512 cycles per k-block that its MMAs take; int8 8192 x 28672 x
-// 8192 in 1.26 ms = 3.05 Pop/s) and, with 8-bit weights, shared memory (96 KB per k-block); 8-bit weights and few rows memory
+// 8192 in 1.28 ms = 3.0 Pop/s, 1.24 - 1.28 by box) and, with 8-bit weights, shared memory (96 KB per k-block); 8-bit weights and few rows memory
 // (28672 x 8192, up to 32 rows: 41 us = 5.7 TB/s); ternary weights and few rows the decode warps' integer instructions: 140 ns
-// per k-block, of which 104 remain without the decoding and 92 without its stores, where memory's 93 are.
+// per k-block, of which 104 remain without the decoding and 92 without its stores, where memory's 93 are; the int8 kernels of
+// 32, 64 and 128 rows spill 32 / 32 / 44 bytes at the 80 registers that 24 warps leave each thread.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -7,9 +7,9 @@
 // only that: L2 is where a predecessor's writes arrive, so weights it has just written are seen all the same - and copies them
 // into shared memory after the wait, while every CTA reads the few rows of X, finds their maxima and quantises them into
 // shared memory for itself: up to TMQ_A8_FUSED_ELEMS elements, 148 times the same 8 KB cost less than a second launch and its hand-over.
-// Then it multiplies with warp-level int8 MMAs, the rows as their eight columns (byte dot products for one row measured 5.9
-// against 6.2 us on 11008 x 4096, 3.2 against 2.8 us on 1024 x 2048).  Sums are exact, so the order of the warps' slices does
-// not show.
+// Then it multiplies with warp-level int8 MMAs, the rows as their eight columns, for one row too: byte dot products took 5.9 us
+// instead of 6.2 on 11008 x 4096 but 3.2 instead of 2.8 on 1024 x 2048, which does not pay for a second form.  (Now 6.4 us for the
+// first, in a graph of such calls.)  Sums are exact, so the order of the warps' slices does not show.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
